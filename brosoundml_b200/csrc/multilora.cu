@@ -1317,11 +1317,13 @@ struct Call {
         a.rng = p.rng;
         a.zero_padding = p.zero_padding;
         a.y = y; a.h = h;
-        const int smem = ((kSmallF + kSmallR) * kSmallPitch + kSmallR * p.rank) * 4;
-        BSML_CUDA(cudaFuncSetAttribute(project_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        auto smem = [](int rank) { return ((kSmallF + kSmallR) * kSmallPitch + kSmallR * rank) * 4; };
+        // (the kernel's limit, the same from every call: two host threads may be here at once)
+        BSML_CUDA(cudaFuncSetAttribute(project_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       smem(kMaxRank)));
         ::bsml::count_launch();
         project_small_kernel<T><<<dim3((unsigned)ceil_div(p.rows, kSmallR), (unsigned)ceil_div(p.cout, kSmallF)),
-                                  2 * kThreads, smem, st>>>(a);
+                                  2 * kThreads, smem(p.rank), st>>>(a);
         BSML_LAUNCH("multilora small");
     }
 

@@ -38,7 +38,8 @@ namespace {
 
 __device__ int g_ml_err = 0;
 
-constexpr int kSmemMax = 232448;      // opt-in dynamic shared memory per block
+constexpr int kSmemMax = 232448;      // opt-in shared memory per block, static and dynamic
+constexpr int kDynMax = kSmemMax - 1024;   // of it dynamic, at most: the kernels' limit, whatever a call takes
 constexpr int kTileA = 16384;         // 128 features x 128 bytes of K
 constexpr int kMaxStages = 12;
 constexpr int kThreads = 320;         // split kernel: TMA warp, MMA warp, 8 epilogue warps
@@ -1177,7 +1178,9 @@ int sm_count() {
 template <class K>
 void launch(K kernel, int grid, int threads, int cluster, int smem, cudaStream_t st, const CUtensorMap (&m)[4],
             const PArgs& a) {
-    BSML_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // the limit belongs to the kernel, not to the call: every call sets the same one, so that calls
+    // from several host threads do not lower each other's
+    BSML_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynMax));
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1287,7 +1290,7 @@ void run(const ProjectTc& p, const Operands& o, cudaStream_t st) {
     const int stage = kTileA + nb * 128;
     // the join's partial sums, and the CUDA cores' products beside them
     const int recv = split && a.splits > 1 ? (a.splits + 1) * a.qpo * 2048 : 0;
-    a.stages = std::min(kMaxStages, (kSmemMax - 2048 - recv) / stage);
+    a.stages = std::min(kMaxStages, (kDynMax - 1024 - recv) / stage);
     const int smem = a.stages * stage + recv + 1024;
     a.idesc = tc::make_idesc(p.dtype == DT_F16 ? 0u : 1u, TR ? 1u : 0u, 0u, split ? 128 : 256, 0);
 

@@ -1,0 +1,51 @@
+"""What the projection of many requests promises beyond single calls of ordinary numbers: calls from
+several host threads, long sums, small numbers, numbers that are not finite, memory."""
+
+import threading
+
+import pytest
+import torch
+
+from brosoundml_b200 import _lib
+from tests import multilora_ref as ref
+from tests.conftest import cuda_available
+from tests.test_gpu_multilora import TYPES, _agree, _expect, _lora, _make, _rng, _run
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not cuda_available(), reason="needs a CUDA device")]
+
+
+@pytest.mark.parametrize("dtype,shapes", [
+    # one kernel each, whose shared memory differs by the rank, and by the columns and parts of a tile
+    ("fp32", [(1, 128, 256, 128, 1, "each"), (1, 128, 256, 1, 1, "each")]),
+    ("bf16", [(16, 1024, 256, 8, 2, "each"), (128, 1024, 1024, 8, 2, "each")])])
+def test_threads_share_a_kernel(dtype, shapes):
+    """Calls of one type and two shapes from several host threads, each on its own stream, are all taken,
+    and are what they are one after the other."""
+    problems = [_make(dtype, *s, seed=i) for i, s in enumerate(shapes)]
+    L, C = _lora(), _lib.lib()
+    want = [L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"]) for c in problems]
+    streams, outs, calls = [torch.cuda.Stream() for _ in range(4)], [], []
+    for i in range(4):
+        c, (M, K, N, R, nA, _) = problems[i % 2], shapes[i % 2]
+        outs.append(torch.zeros_like(want[i % 2]))
+        at = [c[k].data_ptr() for k in ("x", "W", "A", "B", "ids")]
+        calls.append((_lib.BsmlMultiLoraShape(L.DTYPE[TYPES[dtype]], M, K, N, R, nA, 0, 0.0), at[0], K, at[1], None,
+                      at[2], at[3], None, at[4], None, outs[i].data_ptr(), N, None, streams[i].cuda_stream))
+    torch.cuda.synchronize()
+    refused, start = [], threading.Barrier(4)
+
+    def work(i):   # nothing but the calls, which let other threads run
+        start.wait()
+        for _ in range(5000):
+            if C.bsml_multilora_forward(*calls[i]):
+                refused.append(C.bsml_last_error().decode())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused, f"{len(refused)} calls: {refused[0]}"
+    for i in range(4):
+        assert torch.equal(outs[i], want[i % 2])
