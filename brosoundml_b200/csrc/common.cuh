@@ -20,7 +20,9 @@ struct Error : std::runtime_error {
 }
 
 inline void check_cuda(cudaError_t e, const char* where) {
-    if (e != cudaSuccess) fail(where, cudaGetErrorString(e));
+    if (e == cudaSuccess) return;
+    cudaGetLastError();   // reported here, and not by the launch check of this thread's next call
+    fail(where, cudaGetErrorString(e));
 }
 
 #define BSML_CUDA(call) ::bsml::check_cuda((call), #call)

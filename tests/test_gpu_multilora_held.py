@@ -49,3 +49,18 @@ def test_threads_share_a_kernel(dtype, shapes):
     assert not refused, f"{len(refused)} calls: {refused[0]}"
     for i in range(4):
         assert torch.equal(outs[i], want[i % 2])
+
+
+def test_a_refused_call_leaves_nothing_behind():
+    """A call that the device refuses (scratch beyond its memory, before any launch) says so; the next one
+    does not."""
+    c = _make("bf16", 40, 1032, 200, 8, 4, "scattered")
+    want = _run(c)
+    shape = _lib.BsmlMultiLoraShape(1, (1 << 30) - 1, 1032, 200, 128, 4, 0, 0.0)
+    at = [c[k].data_ptr() for k in ("x", "W", "A", "B", "ids")]
+    rc = _lib.lib().bsml_multilora_forward(shape, at[0], 1032, at[1], None, at[2], at[3], None, at[4], None,
+                                           want["y"].data_ptr(), 200, None, torch.cuda.current_stream().cuda_stream)
+    assert rc != 0 and "memory" in _lib.lib().bsml_last_error().decode()
+    got = _run(c)
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
