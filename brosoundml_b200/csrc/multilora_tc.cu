@@ -29,6 +29,7 @@
 
 #include "common.cuh"
 #include "multilora.h"
+#include "multilora_layout.h"
 #include "scalar.cuh"
 #include "tc_ptx.cuh"
 
@@ -1095,46 +1096,23 @@ PFN_cuTensorMapEncodeTiled_v12000 encode() {
     return fn;
 }
 
-// An operand as the kernels read it: planes x rows x cols of 16-bit numbers.
-struct Operand {
-    const void* p = nullptr;
-    int64_t ld = 0, rows = 0, planes = 1;
-    int cols = 0;
-    bool moved = false;       // laid out in scratch
-    int64_t bytes = 0;        // of scratch
-};
-
-Operand operand(const void* p, int64_t ld, int64_t rows, int cols, int dtype) {
-    Operand o;
-    o.p = p;
-    o.rows = rows;
-    o.cols = cols;
-    o.ld = rows > 1 ? ld : round_up(cols, 8);
-    o.moved = dtype == DT_F32 || (reinterpret_cast<uintptr_t>(p) & 15) != 0 || o.ld % 8 != 0;
-    if (o.moved) {
-        o.ld = round_up(cols, 8);
-        o.planes = dtype == DT_F32 ? 3 : 1;
-        o.bytes = round_up(o.planes * o.rows * o.ld * 2, 256);
-    }
-    return o;
-}
-
 struct Operands {
     Operand z, W, Q, P;
     int64_t bytes() const { return z.bytes + W.bytes + Q.bytes + P.bytes; }
 };
 Operands operands(const ProjectTc& p) {
     Operands o;
-    const bool tr = p.transposed;
-    o.z = operand(p.z, p.ldz, p.rows, p.width, p.dtype);
+    const bool tr = p.transposed, f32 = p.dtype == DT_F32;
+    o.z = operand(p.z, p.ldz, p.rows, p.width, f32, false);
     if (p.out) {
         const int64_t q_rows = (int64_t)p.adapters * (tr ? p.rank : p.feats);
-        o.W = operand(p.W, tr ? p.feats : p.width, tr ? p.width : p.feats, tr ? p.feats : p.width, p.dtype);
-        o.Q = operand(p.Q, tr ? p.feats : p.rank, q_rows, tr ? p.feats : p.rank, p.dtype);
+        o.W = operand(p.W, tr ? p.feats : p.width, tr ? p.width : p.feats, tr ? p.feats : p.width, f32, false);
+        o.Q = operand(p.Q, tr ? p.feats : p.rank, q_rows, tr ? p.feats : p.rank, f32, false);
     }
     if (p.P) {
         const int64_t p_rows = (int64_t)p.adapters * (tr ? p.width : p.rank);
-        o.P = operand(p.P, tr ? p.rank : p.width, p_rows, tr ? p.rank : p.width, p.dtype);
+        // (transposed, the thin kernels take its rows of ranks in pieces of 8 or 2)
+        o.P = operand(p.P, tr ? p.rank : p.width, p_rows, tr ? p.rank : p.width, f32, tr);
     }
     return o;
 }

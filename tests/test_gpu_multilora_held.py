@@ -64,3 +64,15 @@ def test_a_refused_call_leaves_nothing_behind():
     got = _run(c)
     for k in want:
         assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("rank", [1, 4, 12])
+@pytest.mark.parametrize("rows", [2, 1500])
+def test_the_smallest_adapter_at_its_buffers_end(dtype, rank, rows):
+    """One adapter of one output, B alone in the last bytes of its buffer, on a 16-byte boundary."""
+    c = _make(dtype, rows, 40, 1, rank, 1, "each")
+    end = torch.zeros(8 * 64, dtype=TYPES[dtype], device="cuda")[:8 + rank]   # (the allocation itself is longer)
+    end[8:] = c["B"].view(-1)
+    c["B"] = end[8:].view(1, 1, rank)
+    _agree(_run(c), _expect(c))
