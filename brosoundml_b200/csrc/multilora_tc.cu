@@ -1103,7 +1103,8 @@ struct Operands {
 Operands operands(const ProjectTc& p) {
     Operands o;
     const bool tr = p.transposed, f32 = p.dtype == DT_F32;
-    o.z = operand(p.z, p.ldz, p.rows, p.width, f32, false);
+    // (fp32's planes of z are for the wide product and the thin one of tiles; rows read z as it is)
+    if (!f32 || p.out || p.P) o.z = operand(p.z, p.ldz, p.rows, p.width, f32, false);
     if (p.out) {
         const int64_t q_rows = (int64_t)p.adapters * (tr ? p.rank : p.feats);
         o.W = operand(p.W, tr ? p.feats : p.width, tr ? p.width : p.feats, tr ? p.feats : p.width, f32, false);

@@ -76,3 +76,16 @@ def test_the_smallest_adapter_at_its_buffers_end(dtype, rank, rows):
     end[8:] = c["B"].view(-1)
     c["B"] = end[8:].view(1, 1, rank)
     _agree(_run(c), _expect(c))
+
+
+def test_the_adapters_gradients_alone_copy_nothing():
+    """fp32 rows read where they stand: without dx the backward is the thin product and the outer ones, and
+    the gradients are what they are beside dx."""
+    L, C = _lora(), _lib.lib()
+    c = _make("fp32", 60, 640, 520, 8, 3, "scattered")
+    want = _run(c)
+    n = C.bsml_launch_count()
+    got = L.multi_lora_backward(c["dy"], c["x"], c["W"], c["A"], c["B"], c["ids"], want["h"], scale=c["scale"],
+                                want_dx=False)
+    assert C.bsml_launch_count() - n == 2
+    assert torch.equal(got["dA"], want["dA"]) and torch.equal(got["dB"], want["dB"])
