@@ -285,14 +285,14 @@ def multi_lora_backward(dy, x, W, A, B, row_ids, h, scale=None, dropout: float =
     """Gradients of :func:`multi_lora_forward` (``bsml_multilora_backward``) from dy (rows, cout), with the
     forward's arguments and its ``h``: a dict of dx (rows, cin), dA and dB (the layouts and type of A and B,
     overwritten; zero for an adapter without rows). W is frozen. dx, dA, dB may be given as preallocated
-    outputs; a given dx keeps its padding rows, a new one has zeros there."""
+    outputs; a given dx keeps its padding rows, a new one has zeros there. x is read for dA alone and ``h``
+    for dB alone: either may be None where that is not wanted."""
     (rows, _), dtype, device = _matrix("dy", dy)
     shape, cin, cout, rank, at_W, at_A, at_B, ids, scale, rng = _adapter_args(
         W, A, B, row_ids, scale, dropout, rng, dx is None, rows, dtype, device)
     at_dy, lddy = _rows("dy", dy, (rows, cout), dtype, device)
-    at_x, ldx = _rows("x", x, (rows, cin), dtype, device)
-    at_dx = at_dA = at_dB = None
-    lddx = 0
+    at_x = at_h = at_dx = at_dA = at_dB = None
+    ldx = lddx = 0
     if dx is not None:
         at_dx, lddx = _rows("dx", dx, (rows, cin), dtype, device)
     elif want_dx:
@@ -308,9 +308,12 @@ def multi_lora_backward(dy, x, W, A, B, row_ids, h, scale=None, dropout: float =
     elif want_adapters:
         dB = torch.empty_like(B)
         at_dB = dB.data_ptr()
-    h = _whole("h", h, (rows, rank), torch.float32, device)
+    if x is not None or dA is not None:
+        at_x, ldx = _rows("x", x, (rows, cin), dtype, device)
+    if h is not None or dB is not None:
+        at_h = _whole("h", h, (rows, rank), torch.float32, device)
     _call("bsml_multilora_backward", device, shape, at_dy, lddy, at_x, ldx, at_W, at_A, at_B, scale, ids, rng,
-          h, at_dx, lddx, at_dA, at_dB)
+          at_h, at_dx, lddx, at_dA, at_dB)
     return dict(dx=dx, dA=dA, dB=dB)
 
 

@@ -437,7 +437,8 @@ int bsml_multilora_forward(const bsml_multilora_shape* shape, const void* x, int
 /* W is frozen. dx (rows, cin) with row stride lddx, padding rows as in the forward;
  * dA, dB (the layouts of A, B; overwritten, zero for an adapter without rows), summed
  * over an adapter's rows in an order that depends on the arguments alone. Each may be
- * NULL. h is the forward's (read for dB); the other arguments as in the forward. */
+ * NULL. x is read for dA alone, h (the forward's) for dB alone: NULL where that is not
+ * wanted. The other arguments as in the forward. */
 int bsml_multilora_backward(const bsml_multilora_shape* shape, const void* dy, int64_t lddy, const void* x,
                             int64_t ldx, const void* W, const void* A, const void* B, const float* scale,
                             const int* row_ids, const uint64_t* rng, const float* h, void* dx, int64_t lddx, void* dA,

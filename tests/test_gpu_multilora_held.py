@@ -89,3 +89,26 @@ def test_the_adapters_gradients_alone_copy_nothing():
                                 want_dx=False)
     assert C.bsml_launch_count() - n == 2
     assert torch.equal(got["dA"], want["dA"]) and torch.equal(got["dB"], want["dB"])
+
+
+@pytest.mark.parametrize("M", [3, 700])
+def test_gradients_need_only_their_own_operands(M):
+    """dx without x and h; dA without h, dB without x: what all together give."""
+    L = _lora()
+    c = _make("bf16", M, 640, 1030, 16, 3, "runs", seed=5)
+    want = _run(c)
+    args, kw = (c["W"], c["A"], c["B"], c["ids"]), dict(scale=c["scale"])
+    got = L.multi_lora_backward(c["dy"], None, *args, None, want_adapters=False, **kw)
+    assert torch.equal(got["dx"], want["dx"]) and got["dA"] is None and got["dB"] is None
+    got = L.multi_lora_backward(c["dy"], c["x"], *args, None, want_dx=False, want_adapters=False,
+                                dA=torch.empty_like(c["A"]), **kw)
+    assert torch.equal(got["dA"], want["dA"]) and got["dB"] is None
+    got = L.multi_lora_backward(c["dy"], None, *args, want["h"], want_dx=False, want_adapters=False,
+                                dB=torch.empty_like(c["B"]), **kw)
+    assert torch.equal(got["dB"], want["dB"]) and got["dA"] is None
+    with pytest.raises(TypeError, match="x: "):
+        L.multi_lora_backward(c["dy"], None, *args, want["h"], **kw)
+    with pytest.raises(TypeError, match="h: "):
+        L.multi_lora_backward(c["dy"], c["x"], *args, None, **kw)
+    with pytest.raises(ValueError, match="x: "):
+        L.multi_lora_backward(c["dy"], c["x"][:, :32], *args, None, want_adapters=False, **kw)
