@@ -191,6 +191,7 @@ SIGNATURES = {
     "bsml_convlora_load": ([_P, ctypes.c_char_p], _I),
     "bsml_multilora_forward": ([_MS, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P, _P], _I),
     "bsml_multilora_backward": ([_MS, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P, _P, _P], _I),
+    "bsml_multilora_release_scratch": ([], _I),
     "bsml_dropout_forward": ([_I, _P, _L, _P, _L, _I, _I, _D, _P, _P, _L, _P], _I),
     "bsml_dropout_backward": ([_I, _P, _L, _I, _I, _D, _P, _P, _L, _P], _I),
     "bsml_lora_save_state": ([_P, ctypes.c_char_p], _I),

@@ -899,6 +899,10 @@ int bsml_multilora_backward(const bsml_multilora_shape* s, const void* dy, int64
     });
 }
 
+int bsml_multilora_release_scratch(void) {
+    return guarded([&] { bsml::multilora_release_scratch(); });
+}
+
 int bsml_dropout_forward(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, int rows, int cols,
                          double p, const uint64_t* rng, void* y, int64_t ldy, void* stream) {
     return guarded([&] {

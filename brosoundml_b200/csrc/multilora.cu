@@ -1149,12 +1149,23 @@ struct Scratch {
     ~Scratch() {
         if (p) cudaFreeAsync(p, st);
     }
-    static cudaMemPool_t pool() {
-        static std::mutex mu;
-        static cudaMemPool_t pools[64] = {};
+    inline static std::mutex mu;
+    inline static cudaMemPool_t pools[64] = {};
+    static int device() {
         int dev = 0;
         BSML_CUDA(cudaGetDevice(&dev));
         if (dev >= 64) fail("multilora", "device above 63");
+        return dev;
+    }
+    // What no call uses any more, back to the device (and what graphs that are gone have left)
+    static void release() {
+        const int dev = device();
+        std::lock_guard<std::mutex> lock(mu);
+        if (pools[dev]) BSML_CUDA(cudaMemPoolTrimTo(pools[dev], 0));
+        BSML_CUDA(cudaDeviceGraphMemTrim(dev));
+    }
+    static cudaMemPool_t pool() {
+        const int dev = device();
         std::lock_guard<std::mutex> lock(mu);
         if (!pools[dev]) {
             cudaMemPoolProps props = {};
@@ -1420,6 +1431,8 @@ struct Call {
 };
 
 }  // namespace
+
+void multilora_release_scratch() { Scratch::release(); }
 
 void multilora_forward(const MultiLora& p, const void* x, int64_t ldx, const void* bias, void* y, int64_t ldy,
                        float* h, cudaStream_t st) {

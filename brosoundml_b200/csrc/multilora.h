@@ -32,6 +32,8 @@ void multilora_forward(const MultiLora& p, const void* x, int64_t ldx, const voi
 // dB_a = sum dy h^T. Each output nullable.
 void multilora_backward(const MultiLora& p, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* h,
                         void* dx, int64_t lddx, void* dA, void* dB, cudaStream_t st);
+// Gives the current device's scratch that no call uses any more back to it.
+void multilora_release_scratch();
 
 // y = residual + keep / (1 - p) * x over (rows, cols); residual nullable, y may be x or residual.
 void dropout(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy, int rows,

@@ -317,6 +317,13 @@ def multi_lora_backward(dy, x, W, A, B, row_ids, h, scale=None, dropout: float =
     return dict(dx=dx, dA=dA, dB=dB)
 
 
+def release_scratch() -> None:
+    """Gives back to the current device the scratch that no call of :func:`multi_lora_forward` or
+    :func:`multi_lora_backward` uses any more (``bsml_multilora_release_scratch``); later calls take it anew."""
+    torch.cuda.synchronize()
+    _lib.check(_lib.lib().bsml_multilora_release_scratch())
+
+
 def dropout_forward(x, p: float, rng, residual=None, y=None):
     """``residual + keep / (1 - p) * x`` (``bsml_dropout_forward``) over x (rows, cols), whose rows may lie in a
     wider tensor. ``rng``: int64 {seed, offset} on the device; the mask is a function of it, the row and the

@@ -420,8 +420,8 @@ int bsml_convlora_load(bsml_convlora* l, const char* path);
  * wider matrix). Where an infinity enters a sum of fp32 operands (which run as bf16
  * planes) or of dA and dB, the sum may be NaN instead of an infinity. The calls take
  * stream-ordered scratch of their own: none is shared between calls, streams or
- * captured graphs, and what the largest calls took is kept for later ones. The
- * current device must be the stream's. */
+ * captured graphs, and what the largest calls took is kept for later ones, until
+ * bsml_multilora_release_scratch. The current device must be the stream's. */
 enum { BSML_F32 = 0, BSML_BF16 = 1, BSML_F16 = 2 };
 #define BSML_MULTILORA_MAX_RANK 128
 typedef struct bsml_multilora_shape {
@@ -443,6 +443,9 @@ int bsml_multilora_backward(const bsml_multilora_shape* shape, const void* dy, i
                             int64_t ldx, const void* W, const void* A, const void* B, const float* scale,
                             const int* row_ids, const uint64_t* rng, const float* h, void* dx, int64_t lddx, void* dA,
                             void* dB, void* stream);
+/* Gives back to the current device the scratch that no call uses any more. What calls
+ * in flight use stays (synchronise first to have it all). Not during a capture. */
+int bsml_multilora_release_scratch(void);
 
 /* Dropout with a mask that is never stored (no counterpart in the reference):
  * y = residual + keep / (1 - p) * x over (rows, cols) with row strides ldx, ldr, ldy

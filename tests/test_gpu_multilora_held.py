@@ -112,3 +112,17 @@ def test_gradients_need_only_their_own_operands(M):
         L.multi_lora_backward(c["dy"], c["x"], *args, None, **kw)
     with pytest.raises(ValueError, match="x: "):
         L.multi_lora_backward(c["dy"], c["x"][:, :32], *args, None, want_adapters=False, **kw)
+
+
+def test_scratch_comes_back():
+    """The planes of a large fp32 weight are the device's again; the next call takes them anew."""
+    L = _lora()
+    c = _make("fp32", 2, 4096, 8192, 8, 2, "each")
+    want = _run(c)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    L.release_scratch()
+    assert torch.cuda.mem_get_info()[0] - before >= 3 * 2 * 4096 * 8192
+    got = _run(c)
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
