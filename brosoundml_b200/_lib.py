@@ -102,6 +102,7 @@ SIGNATURES = {
     "bsml_decoder_decode": ([_P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P], _I),
     "bsml_decoder_workspace_bytes": ([_P], _L),
     "bsml_selftest_bounded_wait": ([_P], _I),
+    "bsml_selftest_multilora_wait": ([_P], _I),
     "bsml_st_open": ([ctypes.c_char_p, ctypes.POINTER(_P)], _I),
     "bsml_st_close": ([_P], None),
     "bsml_st_count": ([_P, ctypes.POINTER(_I)], _I),

@@ -13,6 +13,7 @@
 #include "convlora.h"
 #include "lora.h"
 #include "multilora.h"
+#include "multilora_tc.h"
 #include "nccl_dl.h"
 #include "safetensors.h"
 
@@ -426,6 +427,10 @@ int bsml_device_error(void) {
     int v = 0;
     const int rc = guarded([&] { v = bsml::tc_error_flag(); });
     return rc ? rc : v;
+}
+
+int bsml_selftest_multilora_wait(void* stream) {
+    return guarded([&] { bsml::multilora_wait_selftest(S(stream)); });
 }
 
 int bsml_selftest_bounded_wait(void* stream) {

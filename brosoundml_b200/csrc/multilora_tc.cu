@@ -37,7 +37,12 @@ namespace bsml {
 
 namespace {
 
+// The code of a bounded wait that ran out, for the host (multilora_error_flag). Waits look at a word
+// of their own block's, so that one which ran out ends its block's others early, and no later call's.
 __device__ int g_ml_err = 0;
+__device__ __forceinline__ void report(int gave_up) {
+    if (gave_up != tc::TC_OK) atomicCAS(&g_ml_err, tc::TC_OK, gave_up);
+}
 
 constexpr int kSmemMax = 232448;      // opt-in shared memory per block, static and dynamic
 constexpr int kDynMax = kSmemMax - 1024;   // of it dynamic, at most: the kernels' limit, whatever a call takes
@@ -446,8 +451,9 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
     uint8_t* smem = align1024(smem_raw);
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf[2], acce[2], mdone;
     __shared__ uint32_t tslot;
+    __shared__ int gave_up;
     __shared__ Runs runs[2];
-    int* err = &g_ml_err;
+    int* err = &gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool leader = tc::elect_one();
     const uint32_t rank = tc::cluster_ctarank();
@@ -465,6 +471,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
             tc::mbar_init(&acce[s], 2 * kPairEpi<T>);
         }
         tc::mbar_init(&mdone, 1);
+        gave_up = tc::TC_OK;
         tc::fence_barrier_init();
         tc::prefetch_tmap(&mW);
         tc::prefetch_tmap(&mZ);
@@ -726,6 +733,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
     __syncthreads();
     tc::cluster_sync();   // no CTA leaves while its peer's MMAs, copies or arrivals may reach it
     tc::tc_fence_after();
+    if (threadIdx.x == 0) report(gave_up);
     if (warp == 1) tc::tmem_dealloc_pair(tbase, 512);
 }
 
@@ -745,8 +753,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = align1024(smem_raw);
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf;
     __shared__ uint32_t tslot;
+    __shared__ int gave_up;
     __shared__ Runs runs[2];
-    int* err = &g_ml_err;
+    int* err = &gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool leader = tc::elect_one();
     const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
@@ -767,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&empty[s], 1);
         }
         tc::mbar_init(&accf, 1);
+        gave_up = tc::TC_OK;
         tc::fence_barrier_init();
         tc::fence_async_shared();
         for (int c = 0; c < head; ++c) {
@@ -976,6 +986,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc::cluster_sync();
     tc::tc_fence_after();
+    if (threadIdx.x == 0) report(gave_up);
     if (warp == 1) tc::tmem_dealloc(tbase, DROP ? 256 : 128);
     if (warp >= 2 && a.splits > 1) {
         const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
@@ -1348,6 +1359,24 @@ void project_tc(const ProjectTc& p, void* scratch, cudaStream_t st) {
     if (p.dtype == DT_F32) run_type<float>(p, o, st);
     else if (p.dtype == DT_BF16) run_type<__nv_bfloat16>(p, o, st);
     else run_type<__half>(p, o, st);
+}
+
+__global__ void multilora_wait_selftest_kernel() {
+    __shared__ uint64_t bar;
+    __shared__ int gave_up;
+    if (threadIdx.x == 0) {
+        tc::mbar_init(&bar, 1);
+        tc::fence_barrier_init();
+        gave_up = tc::TC_OK;
+        tc::mbar_wait(&bar, 0, &gave_up, tc::TC_ERR_WAIT_FULL);
+        report(gave_up);
+    }
+}
+
+void multilora_wait_selftest(cudaStream_t st) {
+    ::bsml::count_launch();
+    multilora_wait_selftest_kernel<<<1, 32, 0, st>>>();
+    BSML_LAUNCH("multilora_wait_selftest_kernel");
 }
 
 int multilora_error_flag() {

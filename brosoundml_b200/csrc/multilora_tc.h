@@ -80,5 +80,7 @@ void project_tc(const ProjectTc& p, void* scratch, cudaStream_t st);
 
 // Reads and clears the error word of this file's bounded waits.
 int multilora_error_flag();
+// A wait that runs out, on a barrier that nothing completes.
+void multilora_wait_selftest(cudaStream_t st);
 
 }  // namespace bsml

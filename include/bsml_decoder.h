@@ -421,7 +421,9 @@ int bsml_convlora_load(bsml_convlora* l, const char* path);
  * planes) or of dA and dB, the sum may be NaN instead of an infinity. The calls take
  * stream-ordered scratch of their own: none is shared between calls, streams or
  * captured graphs, and what the largest calls took is kept for later ones, until
- * bsml_multilora_release_scratch. The current device must be the stream's. */
+ * bsml_multilora_release_scratch. The current device must be the stream's. Where a
+ * bounded wait of the tensor-core kernels ran out (2 s), the call's outputs are not
+ * complete: bsml_device_error tells. Later calls are not affected by it. */
 enum { BSML_F32 = 0, BSML_BF16 = 1, BSML_F16 = 2 };
 #define BSML_MULTILORA_MAX_RANK 128
 typedef struct bsml_multilora_shape {
@@ -479,6 +481,9 @@ int bsml_debug_bounds(int* record);
  * whose bounded wait, on a barrier nothing completes, gives up after about 2 s
  * and leaves code 1 (wait for data) in the error word; the context stays usable. */
 int bsml_selftest_bounded_wait(void* stream);
+/* The same for the projection of many requests, whose later calls run as ever while
+ * the code stands. */
+int bsml_selftest_multilora_wait(void* stream);
 
 /* Conv1d forward (modules.cpp:103-108): x (B, Ci, L) -> y (B, Co, Lo). bias may be NULL. */
 int bsml_conv1d_forward(const float* x, int B, int Ci, int L, const float* W, const float* bias, int Co, int k,

@@ -126,3 +126,18 @@ def test_scratch_comes_back():
     got = _run(c)
     for k in want:
         assert torch.equal(got[k], want[k]), k
+
+
+def test_a_wait_that_ran_out_is_told_and_spoils_no_later_call():
+    """The code of an expired wait stands until it is read; the calls in between are what they were."""
+    C = _lib.lib()
+    problems = [_make("bf16", *s) for s in ((3000, 264, 2056, 8, 9, "short"), (16, 2056, 384, 8, 16, "each"))]
+    want = [_run(c) for c in problems]
+    assert C.bsml_device_error() == 0
+    _lib.check(C.bsml_selftest_multilora_wait(torch.cuda.current_stream().cuda_stream))
+    got = [_run(c) for c in problems]
+    assert C.bsml_device_error() == 1
+    for g, w in zip(got, want):
+        for k in w:
+            assert torch.equal(torch.nan_to_num(g[k]), torch.nan_to_num(w[k])), k
+    assert C.bsml_device_error() == 0
