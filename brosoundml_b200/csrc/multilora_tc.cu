@@ -6,8 +6,9 @@
 // of 16 or 32 rows. Where prompts meet inside a group, each row's parts lie in the columns of
 // its slot (the ordinal of its run of rows in 32 rows; zero in the other slots), so one MMA a
 // slot adds each adapter to its own rows, and zeros to the others. Zeros times an infinity or
-// a NaN of a foreign adapter would be NaN: a value of such a group that is not finite is made
-// again by itself (redo). Groups of more runs than slots (single tokens of many requests) get
+// a NaN of a foreign adapter would be NaN. So such a group keeps its low-rank product in an
+// accumulator of its own, where what is not finite is made again alone on the CUDA cores, at the cost of
+// its rank numbers and not of the shared product's width. Groups of more runs than slots (single tokens of many requests) get
 // their products on the CUDA cores in the epilogue, where a lane owns a feature and reads its
 // own contiguous piece of Q_a. Adapters and rows so never meet.
 //
@@ -77,9 +78,8 @@ struct PArgs {
     const RowGroup* groups;
     const uint8_t* wide;
     const float* t;
-    const void *z, *W, *Q;       // as the caller has them
-    int64_t ldz;
-    int width, part_cols;        // part_cols: of one slot
+    const void* Q;               // as the caller has it
+    int part_cols;               // of one slot
     const void* bias;
     DropProb drop;
     const uint64_t* rng;
@@ -154,14 +154,17 @@ __device__ __forceinline__ TileRows tile_rows(const PArgs& a, const RawRows& raw
 
 // Whether the group's low-rank product is the MMAs' work.
 __device__ __forceinline__ bool by_mma(int gid) { return gid >= 0 || gid == kMixed; }
+// Whether that product has an accumulator of its own where there is no dropout.
+__device__ __forceinline__ bool apart(int gid) { return gid == kMixed; }
 
 // A run of groups of one adapter in one slot: what the issuing threads go through. first: no
-// lower slot has an adapter in these groups.
+// lower slot has an adapter in these groups; own: they are apart().
 constexpr int kMaxGroups = 8;
 struct Run {
     int ad;
     int16_t c0, cols;
-    int16_t slot, first;
+    int16_t slot;
+    int8_t first, own;
 };
 typedef Run Runs[kPartSlots * kMaxGroups];
 // The tile's runs, by slot, then column; returns how many. By a whole warp: lane (slot k, group
@@ -179,13 +182,14 @@ __device__ __forceinline__ int find_runs(Runs& out, const TileRows& rows, int gr
     const uint32_t has = __ballot_sync(all, ad >= 0);
     int low = 0;
     for (int i = 0; i < kPartSlots - 1; ++i) low |= i < k ? has >> (i * kMaxGroups + g) & 1 : 0;
-    const int ad_before = __shfl_up_sync(all, ad, 1), low_before = __shfl_up_sync(all, low, 1);
-    const bool start = ad >= 0 && (g == 0 || ad != ad_before || low != low_before);
+    const int own = apart(__shfl_sync(all, rows.gid, g * (G / 16)));
+    const int kind = low | own << 1, ad_before = __shfl_up_sync(all, ad, 1), kind_before = __shfl_up_sync(all, kind, 1);
+    const bool start = ad >= 0 && (g == 0 || ad != ad_before || kind != kind_before);
     const uint32_t starts = __ballot_sync(all, start);
     if (start) {
         const uint32_t more = (has & ~starts) >> lane >> 1;   // lanes after this one that go on with it
         out[__popc(starts & ((1u << lane) - 1))] =
-            Run{ad, (int16_t)(g * G), (int16_t)(__ffs(~more) * G), (int16_t)k, (int16_t)!low};
+            Run{ad, (int16_t)(g * G), (int16_t)(__ffs(~more) * G), (int16_t)k, (int8_t)!low, (int8_t)own};
     }
     __syncwarp();
     return __popc(starts);
@@ -265,29 +269,13 @@ __device__ __forceinline__ int row_adapter(const PArgs& a, int m) {
     return ad < a.adapters ? max(ad, -1) : -1;
 }
 
-// One value by itself, in fp32 on the CUDA cores: what stands in a mixed group where the sum is
-// not finite, which may be a neighbour's doing. As slow as it looks, for that case alone.
+// Adds to v[j] (j = 0..n-1, n a multiple of kBatch) the low-rank products of rows m0 + j, each of its own
+// adapter, where row j is live and its element kept.
 template <class T, bool TR>
-__device__ __forceinline__ float redo(const PArgs& a, int m, int f, bool keep) {
-    const T *z = (const T*)a.z + m * a.ldz, *W = (const T*)a.W + (TR ? (int64_t)f : (int64_t)f * a.width);
-    float s = 0.f, low = 0.f;
-    for (int k = 0; k < a.width; ++k) s = fmaf(to_f(z[k]), to_f(W[TR ? (int64_t)k * a.feats : k]), s);
-    const int ad = row_adapter(a, m);
-    if (ad >= 0 && keep) {
-        const T* Q = (const T*)a.Q + (TR ? (int64_t)ad * a.rank * a.feats + f : ((int64_t)ad * a.feats + f) * a.rank);
-        for (int r = 0; r < a.rank; ++r)
-            low = fmaf(a.t[(int64_t)m * a.rank + r], to_f(Q[TR ? (int64_t)r * a.feats : r]), low);
-    }
-    return s + low;
-}
-
-// Adds to v[j] (j = 0..15) the low-rank products of rows m0 + j, each of its own adapter, where
-// row j is live and its element kept.
-template <class T, bool TR>
-__device__ __forceinline__ void add_many(const PArgs& a, int m0, uint32_t live, uint32_t keep, int f, float* v) {
+__device__ __forceinline__ void add_many(const PArgs& a, int m0, int n, uint32_t live, uint32_t keep, int f, float* v) {
     if (f >= a.feats) return;
 #pragma unroll 1
-    for (int j0 = 0; j0 < 16; j0 += kBatch) {
+    for (int j0 = 0; j0 < n; j0 += kBatch) {
         int m[kBatch], ad[kBatch];
         float s[kBatch];
 #pragma unroll
@@ -302,52 +290,35 @@ __device__ __forceinline__ void add_many(const PArgs& a, int m0, uint32_t live, 
     }
 }
 
-// What the CUDA cores do to the sums of 16 rows: the products of a group of many adapters, or the
-// values of a mixed one that are not finite. Not inlined: long, and rarely reached.
+// What the CUDA cores do to 16 rows: the products of a group of many adapters. Not inlined: long, and
+// rarely reached.
 template <class T, bool TR>
-__device__ __noinline__ void fix_rows(const PArgs& a, bool many, int m0, uint32_t live, uint32_t keep, int f,
-                                      float* v) {
-    if (many) {
-        add_many<T, TR>(a, m0, live, keep, f, v);
-    } else if (f < a.feats) {
-        for (int j = 0; j < 16; ++j)
-            if ((live >> j & 1) && !isfinite(v[j])) v[j] = redo<T, TR>(a, m0 + j, f, keep >> j & 1);
-    }
+__device__ __noinline__ void many_rows(const PArgs& a, int m0, uint32_t live, uint32_t keep, int f, float* v) {
+    add_many<T, TR>(a, m0, 16, live, keep, f, v);
 }
-
-// v: the sums of 16 rows from m0 for feature f, to the output (and before it what the CUDA cores
-// add). rows: this warp's rows of the tile, g: the group of 16 in it. Rows that are all live are
-// stored without tests, which cost as much as all the rest. (What spills here goes to L2, the L1
-// being shared memory: 16 epilogue warps of fewer registers, two groups a turn and calls that
-// are not inlined were all slower.)
+// Low-rank products of n rows of a mixed group: those not finite, which may be a neighbour's doing,
+// by themselves. (At most the work of a group of many adapters, whatever stands in the operands: the
+// MMAs wait for it, and their waits are bounded.)
 template <class T, bool TR>
-__device__ __forceinline__ void finish_rows(const PArgs& a, const TileRows& rows, int g, int gid, int m0, int f,
-                                            uint32_t keep, float bias, float (&v)[16]) {
-    const uint32_t bits = __shfl_sync(0xffffffffu, rows.rows, g), live = bits & 0xFFFFu, pad = bits >> 16;
-    bool fix = gid == kMany;
-    if (gid == kMixed)
+__device__ __noinline__ void own_rows(const PArgs& a, int m0, int n, uint32_t live, int f, float* e) {
+    float w[16] = {};
+    add_many<T, TR>(a, m0, n, live, 0xFFFFu, f, w);
+    for (int j = 0; j < n; ++j)
+        if (!isfinite(e[j])) e[j] = w[j];
+}
+template <class T, bool TR, int N>
+__device__ __forceinline__ void own_low(const PArgs& a, int gid, int m0, uint32_t live, int f, float (&e)[N]) {
+    if (gid != kMixed) return;
+    bool bad = false;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) fix |= !isfinite(v[j]);
-    if (fix) {
-        float w[16];
+    for (int j = 0; j < N; ++j) bad |= !isfinite(e[j]);
+    if (!bad) return;
+    float w[N];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = v[j];
-        fix_rows<T, TR>(a, gid == kMany, m0, live, keep, f, w);
+    for (int j = 0; j < N; ++j) w[j] = e[j];
+    own_rows<T, TR>(a, m0, N, live, f, w);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = w[j];
-    }
-    if (f >= a.feats) return;
-    T* o = (T*)a.out + (int64_t)m0 * a.ldo + f;
-    if (live == 0xFFFFu) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j, o += a.ldo) *o = from_f<T>(v[j] + bias);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j, o += a.ldo) {
-        if (live >> j & 1) *o = from_f<T>(v[j] + bias);
-        else if (a.zero_padding && (pad >> j & 1)) *o = from_f<T>(0.f);
-    }
+    for (int j = 0; j < N; ++j) e[j] = w[j];
 }
 
 // Bits j of the result (j = 0..15): column c0 + j of feature f is kept. Lanes 8i..8i+7 of a
@@ -362,6 +333,55 @@ __device__ __forceinline__ uint32_t keep_columns(const PArgs& a, int m0, int f, 
     for (int j = 0; j < 16; ++j)
         keep |= (__shfl_sync(0xffffffffu, mine[j >> 3], (lane & 24) | (j & 7)) >> (lane & 7) & 1u) << j;
     return keep;
+}
+
+// Sums of 16 rows from m0 for feature f to the output. Rows that are all live are stored without tests,
+// which cost as much as all the rest.
+template <class T>
+__device__ __forceinline__ void store_rows(const PArgs& a, uint32_t live, uint32_t pad, int m0, int f, float bias,
+                                           const float (&v)[16]) {
+    if (f >= a.feats) return;
+    T* o = (T*)a.out + (int64_t)m0 * a.ldo + f;
+    if (live == 0xFFFFu) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, o += a.ldo) *o = from_f<T>(v[j] + bias);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j, o += a.ldo) {
+        if (live >> j & 1) *o = from_f<T>(v[j] + bias);
+        else if (a.zero_padding && (pad >> j & 1)) *o = from_f<T>(0.f);
+    }
+}
+
+// v: the sums of 16 rows from m0 for feature f, to the output (and before it what the CUDA cores
+// add). rows: this warp's rows of the tile, g: the group of 16 in it. (What spills here goes to L2, the L1
+// being shared memory: 16 epilogue warps of fewer registers, two groups a turn and calls that
+// are not inlined were all slower.)
+template <class T, bool TR>
+__device__ __forceinline__ void finish_rows(const PArgs& a, const TileRows& rows, int g, int gid, int m0, int f,
+                                            uint32_t keep, float bias, float (&v)[16]) {
+    const uint32_t bits = __shfl_sync(0xffffffffu, rows.rows, g), live = bits & 0xFFFFu, pad = bits >> 16;
+    if (gid == kMany) {
+        float w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = v[j];
+        many_rows<T, TR>(a, m0, live, keep, f, w);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = w[j];
+    }
+    store_rows<T>(a, live, pad, m0, f, bias, v);
+}
+// Rows of a mixed group whose low-rank product came out not finite: the shared sums from TMEM, and every
+// row's own product on the CUDA cores. Whole warp.
+template <class T, bool TR, bool DROP>
+__device__ __noinline__ void again(const PArgs& a, uint32_t bits, uint32_t taddr, int m0, int f, int lane, float bias) {
+    float v[16];
+    tc::tmem_ld16(taddr, v);
+    uint32_t keep = 0xFFFFu;
+    if (DROP) keep = keep_columns(a, m0, f, lane, load_rng(a.rng));
+    add_many<T, TR>(a, m0, 16, bits & 0xFFFFu, keep, f, v);
+    store_rows<T>(a, bits & 0xFFFFu, bits >> 16, m0, f, bias, v);
 }
 
 // Producer side of one stage: A block (128 features of this CTA) and nb rows of the B operand.
@@ -423,6 +443,22 @@ constexpr int kMaxColumns = DROP && sizeof(T) == 4 ? 160 : 256;
 template <class T>
 constexpr int kPairEpi = sizeof(T) == 4 ? 16 : 8;
 
+// A tile's sums go to the accumulators in turn, whose uses every role counts alike: `at` is the next one, bit i
+// of `uses` whether i was used an odd number of times. A tile with groups apart() also uses, for these, the one after its last
+// sum's, and the next tile's first sum then uses that.
+struct Turns {
+    int at = 0;
+    uint32_t uses = 0;
+    __device__ __forceinline__ uint32_t phase(int i) const { return uses >> i & 1; }
+    __device__ __forceinline__ void used(int i) { uses ^= 1u << i; }
+    template <int B>
+    __device__ __forceinline__ int next() {
+        const int i = at;
+        at = B == 1 ? 0 : at ^ 1;
+        return i;
+    }
+};
+
 struct TilePos {
     int f, m;
 };
@@ -437,6 +473,8 @@ __device__ __forceinline__ TilePos tile_pos(const PArgs& a, int tile) {
 // take 96. Accumulators are double buffered in TMEM, so a tile's stores run under the next
 // tile's MMAs. With dropout (backward) the low-rank product has an accumulator of its own,
 // because its mask does not apply to the shared one (kSums); the masks are made while the sums are.
+// Without, groups where adapters meet inside an MMA's columns have it in the accumulator of the next tile's
+// shared sum, and the epilogue adds it to the tile's own, in TMEM, before anything else (Turns).
 // Bound by the tensor pipe at 256 columns (about 560 cycles for 64 columns of K, of which 512 are
 // MMAs), by L2's operand rate below: 8192 x 4096 x 4096 bf16 187 us alone (1.47 PFLOP/s; the low-rank
 // steps of 16 ranks and 8 prompts add 3), 203 with dropout; 2048 x 2048 x 2048 fp32 106 us.
@@ -546,36 +584,40 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
             // ── MMA issuer (the even CTA)
             Ring r;
             bool ok = true, dep = false;
-            int n = 0;
-            for (int tile = pair; ok && tile < n_tiles; tile += pairs, ++n) {
+            Turns u;
+            auto vacant = [&](int i) {   // accumulator i is read out
+                return tc::mbar_wait(&acce[i], u.phase(i) ^ 1, err, tc::TC_ERR_WAIT_ACC);   // (at first: at once)
+            };
+            for (int tile = pair; ok && tile < n_tiles; tile += pairs) {
                 const int m0 = tile_pos(a, tile).m * a.np;
-                const int last = (n + 1) * sums - 1;   // the tile's last sum, counted over all tiles
-                const uint32_t d = tbase + (uint32_t)(last % B * a.np), de = DROP ? tbase + (uint32_t)(B * a.np) : d;
                 RawRows raw;
                 if (dep) raw = load_rows(a, m0, lane);
-                if (leader) {
-                    const uint32_t idesc = idesc_n(a.idesc, a.np);
-                    for (int c = 0; ok && c < steps; ++c) {
-                        const int in = F32 ? c % kPromote : c, g = n * sums + (F32 ? c / kPromote : 0), buf = g % B;
-                        if (in == 0 && g >= B)
-                            ok = tc::mbar_wait(&acce[buf], (g / B - 1) & 1, err, tc::TC_ERR_WAIT_ACC);
-                        ok = ok && tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        const uint32_t base = tc::smem_u32(smem + r.slot * stage_bytes);
+                int buf = 0;
+                for (int g = 0; g < sums; ++g) {   // (every lane counts, one issues)
+                    buf = u.next<B>();
+                    if (leader && ok) {
+                        const uint32_t idesc = idesc_n(a.idesc, a.np);
+                        const int first = F32 ? g * kPromote : 0, n = F32 ? min(steps - first, kPromote) : steps;
+                        ok = vacant(buf);
+                        for (int c = 0; ok && c < n; ++c) {
+                            ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                            const uint32_t base = tc::smem_u32(smem + r.slot * stage_bytes);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma<true>(tbase + (uint32_t)(buf * a.np), desc_a<TR>(base, k),
-                                      tc::desc_kmajor_sw128(base + kTileA + k * 32), idesc, (in | k) != 0);
-                        commit<true>(&empty[r.slot]);
-                        r.next(a.stages);
-                        if (F32 && in == kPromote - 1 && c + 1 < steps) commit<true>(&accf[buf]);
+                            for (int k = 0; k < 4; ++k)
+                                mma<true>(tbase + (uint32_t)(buf * a.np), desc_a<TR>(base, k),
+                                          tc::desc_kmajor_sw128(base + kTileA + k * 32), idesc, (c | k) != 0);
+                            commit<true>(&empty[r.slot]);
+                            r.next(a.stages);
+                        }
+                        if (ok && g + 1 < sums) commit<true>(&accf[buf]);
                     }
-                    // the low-rank accumulator of the tile before is read out (with one sum, or
-                    // two and more a tile, the last of them waited for that)
-                    if (DROP && B == 2 && ok && n >= 1 && sums == 1)
-                        ok = tc::mbar_wait(&acce[(n - 1) & 1], ((n - 1) >> 1) & 1, err, tc::TC_ERR_WAIT_ACC);
+                    if (g + 1 < sums) u.used(buf);
                 }
+                // the low-rank accumulator of the tile before is read out (with one sum, or with several a
+                // tile, the last of which waited for that)
+                if (DROP && B == 2 && leader && ok && sums == 1) ok = vacant(buf ^ 1);
                 __syncwarp();
                 if (!dep) {
                     tc::grid_dependency_wait();
@@ -584,10 +626,14 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                 }
                 const TileRows rows = tile_rows<WIDE, 32>(a, raw, m0, lane);
                 const int n_runs = find_runs<32>(runs[1], rows, groups, lane);
+                const bool own = !DROP && __any_sync(0xffffffffu, apart(rows.gid));
                 if (leader && ok) {
+                    if (own) ok = vacant(buf ^ 1);
                     for (int i = 0; ok && i < n_runs; ++i) {
-                        const Run u = runs[1][i];
-                        const uint32_t idesc = idesc_n(a.idesc, u.cols);
+                        const Run v = runs[1][i];
+                        const uint32_t idesc = idesc_n(a.idesc, v.cols);
+                        const bool alone = DROP || v.own;   // in an accumulator of its own
+                        const uint32_t d = tbase + (uint32_t)((DROP ? B : v.own ? buf ^ 1 : buf) * a.np + v.c0);
                         for (int e = 0; e < a.n_ext; ++e) {
                             const ExtStage& x = a.ext[e];
                             ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
@@ -595,15 +641,18 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                             tc::tc_fence_after();
                             const uint32_t base = tc::smem_u32(smem + r.slot * stage_bytes);
                             for (int k = 0; k < x.n; ++k)
-                                mma<true>(de + (uint32_t)u.c0, desc_a<TR>(base, x.a[k]),
+                                mma<true>(d, desc_a<TR>(base, x.a[k]),
                                           tc::desc_kmajor_sw128(base + kTileA + x.b[k] * 32), idesc,
-                                          !DROP || !u.first || (e | k) != 0);
+                                          !alone || !v.first || (e | k) != 0);
                             commit<true>(&empty[r.slot]);
                             r.next(a.stages);
                         }
                     }
-                    if (ok) commit<true>(&accf[last % B]);
+                    if (ok) commit<true>(&accf[buf]);
+                    if (ok && own) commit<true>(&accf[buf ^ 1]);
                 }
+                u.used(buf);
+                if (own) u.used(buf ^ 1);
                 ok = __all_sync(0xffffffffu, ok);
             }
             if (!dep) tc::grid_dependency_wait();
@@ -623,74 +672,114 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
         const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
         const uint32_t lead[2] = {tc::map_shared(tc::smem_u32(&acce[0]), 0), tc::map_shared(tc::smem_u32(&acce[1]), 0)};
         bool ok = true;
-        int n = 0;
-        for (int tile = pair; tile < n_tiles; tile += pairs, ++n) {
+        Turns u;
+        for (int tile = pair; tile < n_tiles; tile += pairs) {
             const TilePos at = tile_pos(a, tile);
             const int m0 = at.m * a.np, f = at.f * 256 + (int)rank * 128 + q * 32 + lane;
             const TileRows rows = tile_rows<WIDE, 32>(a, load_rows(a, m0, lane), m0, lane);
             const float bias = a.bias && f < a.feats ? to_f(((const T*)a.bias)[f]) : 0.f;
             const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
+            const bool own = !DROP && __any_sync(0xffffffffu, apart(rows.gid));
+            // groups whose low-rank product is not finite, and their rows once more, with the shared
+            // sums at `column`
+            uint32_t bad = 0;
+            auto finish_again = [&](int column) {
+#pragma unroll 1
+                for (int g = h; g * 16 < a.np; g += HG) {
+                    const uint32_t bits = __shfl_sync(0xffffffffu, rows.rows, g);
+                    if (bad >> g & 1)
+                        again<T, TR, DROP>(a, bits, trow + (uint32_t)(column + g * 16), m0 + g * 16, f, lane, bias);
+                }
+            };
             auto finish = [&](int g, int gid, uint32_t keep, float (&v)[16]) {
                 finish_rows<T, TR>(a, rows, g, gid, m0 + g * 16, f, keep, bias, v);
             };
             auto keep_of = [&](int g, int gid) {
                 return DROP && gid != kNone ? keep_columns(a, m0 + g * 16, f, lane, key) : 0xFFFFu;
             };
-            auto wait_sum = [&](int s) {
+            auto wait_sum = [&](int i) {   // of accumulator i
                 bool w = true;
-                if (lane == 0) w = tc::mbar_wait(&accf[s % B], (s / B) & 1, err, tc::TC_ERR_WAIT_ACC);
+                if (lane == 0) w = tc::mbar_wait(&accf[i], u.phase(i), err, tc::TC_ERR_WAIT_ACC);
                 const bool got = __shfl_sync(0xffffffffu, w ? 1 : 0, 0) != 0;
                 tc::tc_fence_after();
                 return got;
             };
-            auto release = [&](int s) {
+            auto release = [&](int i) {
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive_cluster(lead[s % B]);
+                if (lane == 0) tc::mbar_arrive_cluster(lead[i]);
+                u.used(i);
             };
             if constexpr (F32) {
                 constexpr int NG = (kMaxColumns<T, DROP> / 16 + HG - 1) / HG;   // this warp's column groups
                 float v[NG][16] = {};
                 uint32_t keep[NG];
-                for (int s = n * sums; ok && s < (n + 1) * sums; ++s) {
-                    ok = wait_sum(s);
+                int buf = 0;
+                for (int s = 0; s < sums; ++s) {
+                    buf = u.next<B>();
+                    ok = wait_sum(buf);
                     if (!ok) break;
-                    const bool end = s == (n + 1) * sums - 1;
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
                         const int g = h + HG * i;
                         if (g * 16 >= a.np) break;
                         // (8 at a time: registers)
-                        uint32_t e[8];
+                        uint32_t x[8];
 #pragma unroll
                         for (int o = 0; o < 16; o += 8) {
-                            tc::tmem_ld8_nowait(trow + (uint32_t)((s & 1) * a.np + g * 16 + o), e);
+                            tc::tmem_ld8_nowait(trow + (uint32_t)(buf * a.np + g * 16 + o), x);
                             tc::tmem_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[i][o + j] += __uint_as_float(e[j]);
-                        }
-                        if (end) {
-                            const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
-                            keep[i] = keep_of(g, gid);
-                            if (DROP && by_mma(gid))
-#pragma unroll
-                                for (int o = 0; o < 16; o += 8) {
-                                    tc::tmem_ld8_nowait(trow + (uint32_t)(B * a.np + g * 16 + o), e);
-                                    tc::tmem_wait_ld();
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        if (keep[i] >> (o + j) & 1) v[i][o + j] += __uint_as_float(e[j]);
-                                }
+                            for (int j = 0; j < 8; ++j) v[i][o + j] += __uint_as_float(x[j]);
                         }
                     }
-                    release(s);
+                    if (s + 1 < sums || own) release(buf);
                 }
+                if (ok && own) ok = wait_sum(buf ^ 1);
                 if (!ok) break;
+                const int low = own ? buf ^ 1 : buf, lowc = (DROP ? B : low) * a.np;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const int g = h + HG * i;
+                    if (g * 16 >= a.np) break;
+                    const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
+                    keep[i] = keep_of(g, gid);
+                    if (!(DROP ? by_mma(gid) : apart(gid))) continue;
+                    uint32_t x[8];
+                    if (gid == kMixed) {
+                        bool b = false;
+#pragma unroll
+                        for (int o = 0; o < 16; o += 8) {
+                            tc::tmem_ld8_nowait(trow + (uint32_t)(lowc + g * 16 + o), x);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) b |= !isfinite(__uint_as_float(x[j]));
+                        }
+                        if (__any_sync(0xffffffffu, b)) {   // the shared sums take its place, for again()
+                            bad |= 1u << g;
+                            tc::tmem_st16(trow + (uint32_t)(lowc + g * 16), v[i]);
+                            continue;
+                        }
+                    }
+#pragma unroll
+                    for (int o = 0; o < 16; o += 8) {
+                        tc::tmem_ld8_nowait(trow + (uint32_t)(lowc + g * 16 + o), x);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (keep[i] >> (o + j) & 1) v[i][o + j] += __uint_as_float(x[j]);
+                    }
+                }
+                if (!bad) release(low);
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     const int g = h + HG * i;
                     if (g * 16 >= a.np) break;
                     finish(g, __shfl_sync(0xffffffffu, rows.gid, g), keep[i], v[i]);
+                }
+                if (bad) {
+                    finish_again(lowc);
+                    release(low);
                 }
             } else {
                 // the masks before the sums are there: 16 bits a group, the first lowest
@@ -706,26 +795,58 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                         const int g = h + HG * i;
                         turn(g * 16 < a.np ? keep_of(g, __shfl_sync(0xffffffffu, rows.gid, g & 31)) : 0u);
                     }
-                ok = wait_sum(n);
+                const int buf = u.next<B>();
+                ok = wait_sum(buf) && (!own || wait_sum(buf ^ 1));
                 if (!ok) break;
+                const uint32_t xcol = trow + (uint32_t)(buf * a.np), ycol = trow + (uint32_t)((DROP ? B : buf ^ 1) * a.np);
+                uint32_t x[16], y[16];
+                float v[16];
+                auto sums_of = [&](int g, bool low) {
+                    tc::tmem_ld16_nowait(xcol + (uint32_t)(g * 16), x);
+                    if (low) tc::tmem_ld16_nowait(ycol + (uint32_t)(g * 16), y);
+                    tc::tmem_wait_ld();
+                };
+                auto broken = [&]() {
+                    bool b = false;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) b |= !isfinite(__uint_as_float(y[j]));
+                    return __any_sync(0xffffffffu, b) != 0;
+                };
+                if (own) {
+                    // the low-rank products that stand apart to the sums, so that the MMAs go on
+#pragma unroll 1
+                    for (int g = h; g * 16 < a.np; g += HG) {
+                        const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
+                        if (!apart(gid)) continue;
+                        sums_of(g, true);
+                        if (broken()) {
+                            bad |= 1u << g;
+                            continue;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(x[j]) + __uint_as_float(y[j]);
+                        tc::tmem_st16(xcol + (uint32_t)(g * 16), v);
+                    }
+                    release(buf ^ 1);
+                }
 #pragma unroll 1
                 for (int g = h; g * 16 < a.np; g += HG) {   // 16 columns at a time
-                    uint32_t x[16], e[16];
-                    float v[16];
                     const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
-                    tc::tmem_ld16_nowait(trow + (uint32_t)(n % B * a.np + g * 16), x);
-                    if (DROP && by_mma(gid)) tc::tmem_ld16_nowait(trow + (uint32_t)(B * a.np + g * 16), e);
-                    tc::tmem_wait_ld();
+                    const bool low = DROP && by_mma(gid);
+                    sums_of(g, low);
                     const uint32_t keep = DROP ? kept[0] & 0xFFFFu : 0xFFFFu;
                     if (DROP) turn(0);
+                    if (low && gid == kMixed && broken()) bad |= 1u << g;
+                    if (bad >> g & 1) continue;
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         v[j] = __uint_as_float(x[j]);
-                        if (DROP && by_mma(gid) && (keep >> j & 1)) v[j] += __uint_as_float(e[j]);
+                        if (low && (keep >> j & 1)) v[j] += __uint_as_float(y[j]);
                     }
                     finish(g, gid, keep, v);
                 }
-                release(n);
+                if (bad) finish_again(buf * a.np);
+                release(buf);
             }
         }
     }
@@ -786,14 +907,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     if (warp == 1) {
-        tc::tmem_alloc(&tslot, DROP ? 256 : 128);
+        tc::tmem_alloc(&tslot, 256);
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
     __syncthreads();
     tc::cluster_sync();   // every CTA of the cluster runs before any writes to its shared memory
     tc::tc_fence_after();
-    const uint32_t tbase = tslot, de = DROP ? tbase + 128 : tbase;
+    const uint32_t tbase = tslot, de = tbase + 128;   // the shared sum; the low-rank product's
 
     // epilogue state that outlives the cluster barrier
     const int q = warp & 3, h = (warp - 2) >> 2;
@@ -878,7 +999,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int k = 0; k < x.n; ++k)
                             mma<false>(de + (uint32_t)u.c0, desc_a<TR>(base, x.a[k]),
                                        tc::desc_kmajor_sw128(base + kTileA + x.b[k] * 32), idesc,
-                                       !DROP || !u.first || (e | k) != 0);
+                                       !u.first || (e | k) != 0);
                         commit<false>(&empty[r.slot]);
                         r.next(a.stages);
                     }
@@ -950,23 +1071,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
             const uint32_t mine = tc::smem_u32(recv) + (uint32_t)((split * a.qpo * 128 + q * 32 + lane) * 16);
             for (int g = h; g < groups; g += 2) {
-                uint32_t v[16], e[16];
+                uint32_t v[16], y[16];
                 const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
-                const bool ext = DROP && split == 0 && by_mma(gid);
+                const uint32_t live = __shfl_sync(0xffffffffu, rows.rows, g) & 0xFFFFu;
+                const bool ext = split == 0 && by_mma(gid);
                 tc::tmem_ld16_nowait(trow + (uint32_t)(g * 16), v);
-                if (ext) tc::tmem_ld16_nowait(trow + (uint32_t)(128 + g * 16), e);
+                if (ext) tc::tmem_ld16_nowait(trow + (uint32_t)(128 + g * 16), y);
                 tc::tmem_wait_ld();
-                const uint32_t keep = ext ? keep_columns(a, m0 + g * 16, f, lane, key) : 0;
+                uint32_t keep = 0xFFFFu;
+                if (DROP && (ext || (a.splits == 1 && gid == kMany))) keep = keep_columns(a, m0 + g * 16, f, lane, key);
                 float s[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    s[j] = __uint_as_float(v[j]);
-                    if (DROP && (keep >> j & 1)) s[j] += __uint_as_float(e[j]);
+                for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(v[j]);
+                if (ext) {
+                    float e[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) e[j] = __uint_as_float(y[j]);
+                    own_low<T, TR>(a, gid, m0 + g * 16, live, f, e);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (keep >> j & 1) s[j] += e[j];
                 }
                 if (a.splits == 1) {   // nothing to join
-                    uint32_t kept = DROP ? keep : 0xFFFFu;
-                    if (DROP && gid == kMany) kept = keep_columns(a, m0 + g * 16, f, lane, key);
-                    finish_rows<T, TR>(a, rows, g, gid, m0 + g * 16, f, kept, bias, s);
+                    finish_rows<T, TR>(a, rows, g, gid, m0 + g * 16, f, keep, bias, s);
                     continue;
                 }
                 int to = g * 4 / a.qpo, at = g * 4 - to * a.qpo;
@@ -987,9 +1114,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::cluster_sync();
     tc::tc_fence_after();
     if (threadIdx.x == 0) report(gave_up);
-    if (warp == 1) tc::tmem_dealloc(tbase, DROP ? 256 : 128);
+    if (warp == 1) tc::tmem_dealloc(tbase, 256);
     if (warp >= 2 && a.splits > 1) {
-        const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
         const bool live_f = f < a.feats;
 #pragma unroll 1
         for (int i = h; i < quads; i += 2) {
@@ -1011,18 +1137,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 v.z += w.z;
                 v.w += w.w;
             }
-            float s[4] = {v.x, v.y, v.z, v.w};
-            if (gid == kMixed && !(isfinite(s[0]) && isfinite(s[1]) && isfinite(s[2]) && isfinite(s[3]))) {
-                float w[16] = {s[0], s[1], s[2], s[3]};
-                uint32_t keep = 0xFu;
-                if (DROP)
-                    for (int j = 0; j < 4; ++j)
-                        if (!(keep_bits(f >> 3, (uint32_t)(m0 + quad * 4 + j), key, a.drop.thr) >> (f & 7) & 1))
-                            keep &= ~(1u << j);
-                fix_rows<T, TR>(a, false, m0 + quad * 4, bits & 0xFu, keep, f, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[j] = w[j];
-            }
+            const float s[4] = {v.x, v.y, v.z, v.w};
             T* o = (T*)a.out + (int64_t)(m0 + quad * 4) * a.ldo + f;
             if ((bits & 0xFu) == 0xFu) {
 #pragma unroll
@@ -1231,8 +1346,8 @@ void run(const ProjectTc& p, const Operands& o, cudaStream_t st) {
     const LowParts lp = low_parts(p.rank, p.dtype);
     make_ext(a, lp, p.dtype == DT_F32 ? 3 : 1);
     a.ids = p.ids; a.groups = p.low.groups; a.wide = p.low.wide; a.t = p.low.t;
-    a.z = p.z; a.ldz = p.ldz; a.W = p.W; a.Q = p.Q; a.bias = p.bias;
-    a.width = p.width; a.part_cols = lp.cols;
+    a.Q = p.Q; a.bias = p.bias;
+    a.part_cols = lp.cols;
     a.drop = p.drop; a.rng = p.rng; a.zero_padding = p.zero_padding;
     a.q_vec = !TR && (reinterpret_cast<uintptr_t>(p.Q) & 15) == 0 && (p.rank * sizeof(T)) % 16 == 0;
     a.t_vec = (reinterpret_cast<uintptr_t>(p.low.t) & 15) == 0 && p.rank % 4 == 0;

@@ -141,3 +141,52 @@ def test_a_wait_that_ran_out_is_told_and_spoils_no_later_call():
         for k in w:
             assert torch.equal(torch.nan_to_num(g[k]), torch.nan_to_num(w[k])), k
     assert C.bsml_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("where", ["W", "x", "A", "B"])
+def test_no_numbers_hold_a_call_up(dtype, where):
+    """A weight, rows or an adapter of NaN among short prompts: the call takes what it takes with ordinary
+    numbers, up to the products of the rows beside that adapter on the CUDA cores (a few times as long; the
+    shared product again for every element would be hundreds). Rows of the others keep their results."""
+    M, W = (2500, 2048) if dtype == "fp32" else (5000, 4096)
+    c = _make(dtype, M, W, W, 8, 5, "short", seed=2)
+    bad = {k: v.clone() for k, v in c.items()}
+    if where in "AB":
+        bad[where][1] = float("nan")
+    elif where == "W":
+        bad["W"].fill_(float("nan"))
+    else:
+        bad["x"][::2] = float("nan")
+        bad["dy"][::2] = float("inf")
+    L = _lora()
+    h = torch.empty(M, 8, device="cuda")
+
+    def run(c):
+        y = L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"], h=h)
+        return y, L.multi_lora_backward(c["dy"], None, c["W"], c["A"], c["B"], c["ids"], None, want_adapters=False)["dx"]
+
+    def time(c):
+        run(c)
+        best = 1e9
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            run(c)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert time(bad) < 20 * time(c)
+    assert _lib.lib().bsml_device_error() == 0
+    clean = c["ids"] >= -1
+    clean &= {"W": c["ids"] < -5, "A": c["ids"] != 1, "B": c["ids"] != 1,
+              "x": (torch.arange(M, device="cuda") % 2 == 1)}[where]
+    want, got = run(c), run(bad)
+    for w, g in zip(want, got):
+        w, g = w[clean].double(), g[clean].double()
+        # both are within the output's rounding and the sums' of the same value
+        assert bool(torch.isfinite(g).all())
+        tol = torch.finfo(c["x"].dtype).eps * w.abs() + 2 * (W + 10) * 2.0**-23 * 4 * W**0.5
+        assert bool(((w - g).abs() <= tol).all())
