@@ -28,13 +28,12 @@ constexpr int kMaxRank = 128;
 
 // ── h and g: rows times an adapter's thin matrix
 // A number as the parts of LowParts: two of its 16-bit type, or three bf16 ones. Each part is
-// the rounded remainder of those before it, a number that is not finite has no remainder. An
-// fp16 number that does not fit is left to the CUDA cores (`wide`), its parts are zero. Two parts
+// the rounded remainder of those before it, a number that is not finite has no remainder. Two parts
 // and not the fp32 number, because the product then needs no accumulator of another type beside
-// the shared projection's: bf16 keeps 16 bits (an output's rounding is 8), fp16 22, or steps of 2^-24
-// where the second part is subnormal (numbers below 1/8; an output's own steps there).
+// the shared projection's: bf16 keeps 16 bits (an output's rounding is 8), fp16 (v: times its row's power of two)
+// 22, or steps of 2^-39 of the row's largest number.
 template <class T>
-__device__ __forceinline__ bool put_parts(uint16_t* row, const LowParts& lp, int r, float v) {
+__device__ __forceinline__ void put_parts(uint16_t* row, const LowParts& lp, int r, float v) {
     if constexpr (!std::is_same<T, __half>::value) {
         for (int i = 0; i < lp.n; ++i) {
             __nv_bfloat16 b = __float2bfloat16_rn(v);
@@ -42,15 +41,20 @@ __device__ __forceinline__ bool put_parts(uint16_t* row, const LowParts& lp, int
             row[i * lp.pitch + r] = __bfloat16_as_ushort(b);
             v = isfinite(v) ? v - __bfloat162float(b) : 0.f;
         }
-        return false;
     } else {
-        const bool wide = !(fabsf(v) <= 65504.f);
-        if (wide) v = 0.f;
         const __half hi = __float2half_rn(v);
         row[r] = __half_as_ushort(hi);
-        row[lp.pitch + r] = __half_as_ushort(__float2half_rn(v - __half2float(hi)));
-        return wide;
+        row[lp.pitch + r] = __half_as_ushort(__float2half_rn(isfinite(v) ? v - __half2float(hi) : 0.f));
     }
+}
+// The biased exponent of the power of two over which the numbers of an fp16 row are held, `most` being the largest
+// finite magnitude of them, and the factor that brings them there (most: to 2^14 .. 2^15, numbers
+// below 2^-112 no further than times 2^126).
+__device__ __forceinline__ int row_power(float most) { return max((int)(__float_as_uint(most) >> 23) - 14, 1); }
+__device__ __forceinline__ float row_factor(int power) { return __uint_as_float((uint32_t)(254 - power) << 23); }
+__device__ __forceinline__ float finite_size(float v) { return isfinite(v) ? fabsf(v) : 0.f; }
+__device__ __forceinline__ float warp_max(float v) {   // of numbers >= 0
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
 
 struct ShrinkArgs {
@@ -93,9 +97,7 @@ __device__ __forceinline__ Rows32 rows32(const ShrinkArgs& a, int64_t m0, int la
     r.slot = row_slot(r.ad, lane);
     return r;
 }
-// wide: this lane's row has numbers that do not fit their parts; check: not known yet, see the rows' bytes.
-__device__ __forceinline__ void put_groups(const ShrinkArgs& a, int64_t m0, const Rows32& r, int lane, bool wide,
-                                           bool check) {
+__device__ __forceinline__ void put_groups(const ShrinkArgs& a, int64_t m0, const Rows32& r, int lane) {
     const uint32_t all = 0xffffffffu, half = lane < 16 ? 0x0000FFFFu : 0xFFFF0000u;
     RowGroup g = {};
 #pragma unroll
@@ -106,8 +108,7 @@ __device__ __forceinline__ void put_groups(const ShrinkArgs& a, int64_t m0, cons
     }
     const int at = lane & 16;
     g.rows = (__ballot_sync(all, r.live) >> at & 0xFFFFu) | __ballot_sync(all, r.pad) >> at << 16;
-    g.many = __ballot_sync(all, r.ad >= 0 && (r.slot >= kPartSlots || wide)) & half;
-    g.check = check;
+    g.many = __ballot_sync(all, r.ad >= 0 && r.slot >= kPartSlots) & half;
     g.without = __ballot_sync(all, r.live && r.ad < 0) & half;
     if ((lane & 15) == 0) a.low.groups[m0 / 16 + (lane >> 4)] = g;
 }
@@ -117,7 +118,7 @@ __device__ __forceinline__ uint16_t* parts_row(const ShrinkArgs& a, int64_t m) {
 // The numbers of a row without an adapter.
 __device__ __forceinline__ void put_none(const ShrinkArgs& a, int64_t m, int tid, int n) {
     for (int r = tid; r < a.rank; r += n) a.low.t[m * a.rank + r] = 0.f;
-    if (a.low.wide && tid == 0) *reinterpret_cast<uint4*>(a.low.wide + m * 16) = make_uint4(0, 0, 0, 0);
+    if (a.low.power && tid == 0) a.low.power[m] = 127;
 }
 // Zeros of a row without an adapter (slot < 0), or around the numbers of the parts in `slot`.
 __device__ __forceinline__ void put_zeros(const ShrinkArgs& a, int64_t m, int slot, int tid, int n) {
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 4) shrink_rows_kernel(const __grid_c
     const Rows32 r32 = rows32(a, m & ~31, lane);
     const int at = (int)(m & 31), ad = __shfl_sync(0xffffffffu, r32.ad, at);
     const int slot = __shfl_sync(0xffffffffu, r32.slot, at);
-    if (at == 0 && blockIdx.y == 0 && warp == 0) put_groups(a, m, r32, lane, false, a.low.wide != nullptr);
+    if (at == 0 && blockIdx.y == 0 && warp == 0) put_groups(a, m, r32, lane);
     if (ad < 0) {
         if (blockIdx.y == 0) put_zeros(a, m, -1, tid, kThreads);
         return;
@@ -277,20 +278,31 @@ __global__ void __launch_bounds__(kThreads, 4) shrink_rows_kernel(const __grid_c
         }
     }
     const int r = r0 + tid;
-    bool wide = false;
-    if (r < r1) {
-        const float h = f * sums[0][r];
-        a.low.t[m * a.rank + r] = h;
-        if (slot < kPartSlots) wide = put_parts<T>(parts_row(a, m) + slot * a.lp.cols, a.lp, r, h);
+    float h = r < r1 ? f * sums[0][r] : 0.f;
+    if (r < r1) a.low.t[m * a.rank + r] = h;
+    if constexpr (std::is_same<T, __half>::value) {
+        // the row's largest number: over the warps, and the cluster of the row's CTAs
+        __shared__ float most[4];
+        if (warp < 4) {
+            const float v = warp_max(finite_size(h));
+            if (lane == 0) most[warp] = v;
+        }
+        const int ctas = (int)gridDim.y;
+        if (ctas > 1) tc::cluster_sync();
+        else __syncthreads();
+        float all = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        if (ctas > 1) {
+            float v = 0.f;   // lane: warp (lane & 3) of CTA lane / 4
+            if (lane < 4 * ctas) v = tc::ld_cluster(tc::map_shared(tc::smem_u32(&most[lane & 3]), lane >> 2));
+            all = warp_max(v);
+            tc::cluster_sync();   // no CTA ends before the others have read it
+        }
+        const int power = row_power(all);
+        h *= row_factor(power);
+        if (blockIdx.y == 0 && tid == 0) a.low.power[m] = (uint8_t)power;
     }
+    if (r < r1 && slot < kPartSlots) put_parts<T>(parts_row(a, m) + slot * a.lp.cols, a.lp, r, h);
     if (blockIdx.y == 0) put_zeros(a, m, slot, tid, kThreads);
-    if (a.low.wide && warp < 4) {
-        // a byte for 8 ranks; the first block writes those past the last rank too
-        const uint32_t any = __ballot_sync(0xffffffffu, wide);
-        const int b = r >> 3;
-        if ((lane & 7) == 0 && (r < r1 || (r1 == a.rank && b < 16)))
-            a.low.wide[m * 16 + b] = (any >> lane & 0xFFu) != 0;
-    }
 }
 
 // Copies from global to shared memory that nothing waits for until copy_async_wait.
@@ -360,7 +372,6 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
     __shared__ float sums[4][TM][RP];
     __shared__ int sid[TM], sslot[TM];   // adapter (-1 for none) and slot of each row
     __shared__ int sad[TM], n_ad;
-    __shared__ int swide[TM];   // 1 where numbers of the row do not fit their parts (set by the row's CTA)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     // With few tiles, a cluster shares one: each CTA sums over its part of the columns, and writes
     // the numbers of every splits-th row.
@@ -375,9 +386,8 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
         if (in) {
             sid[row] = mine;
             sslot[row] = r32.slot;
-            swide[row] = 0;
         }
-        if (!F16 && m0 == m32 && split == 0) put_groups(a, m32, r32, lane, false, false);
+        if (m0 == m32 && split == 0) put_groups(a, m32, r32, lane);
         // the tile's adapters, each where its first row stands
         const int id = in ? mine : -1;
         const uint32_t same = __match_any_sync(0xffffffffu, id);   // by every lane, whatever its row
@@ -544,24 +554,35 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
                 }
                 const float h = f * s;
                 a.low.t[(m0 + row) * a.rank + r] = h;
-                if (sslot[row] < kPartSlots &&
-                    put_parts<T>(parts_row(a, m0 + row) + sslot[row] * a.lp.cols, a.lp, r, h))
-                    swide[row] = 1;
+                if (!F16 && sslot[row] < kPartSlots)
+                    put_parts<T>(parts_row(a, m0 + row) + sslot[row] * a.lp.cols, a.lp, r, h);
             }
             // the sums are read before the next ones, or the CTA's end
             if (splits > 1) tc::cluster_sync();
             else __syncthreads();
         }
     }
-    if constexpr (F16) {   // the groups, now that the rows' numbers are known
-        if (warp == 0 && split == 0) {
-            const uint32_t at = tc::smem_u32(&swide[lane]);
-            const bool apart = n_ad > 0 && splits > 1;
-            const bool wide =
-                (apart ? __float_as_int(tc::ld_cluster(tc::map_shared(at, lane % splits))) : swide[lane]) != 0;
-            put_groups(a, m0, rows32(a, m0, lane), lane, wide, false);
+    if constexpr (F16) {   // the parts, now that every number of the rows is known: a warp a row
+#pragma unroll
+        for (int k = 0; k < TM / 8; ++k) {
+            const int i = warp + 8 * k;
+            if (m0 + i >= a.rows || i % splits != split || sid[i] < 0) continue;
+            float v[kMaxRank / 32], most = 0.f;
+#pragma unroll
+            for (int j = 0; j < kMaxRank / 32; ++j) {
+                const int r = lane + 32 * j;
+                v[j] = r < a.rank ? a.low.t[(m0 + i) * a.rank + r] : 0.f;
+                most = fmaxf(most, finite_size(v[j]));
+            }
+            const int power = row_power(warp_max(most));
+            const float up = row_factor(power);
+            if (lane == 0) a.low.power[m0 + i] = (uint8_t)power;
+            if (sslot[i] < kPartSlots)
+#pragma unroll
+                for (int j = 0; j < kMaxRank / 32; ++j)
+                    if (lane + 32 * j < a.rank)
+                        put_parts<T>(parts_row(a, m0 + i) + sslot[i] * a.lp.cols, a.lp, lane + 32 * j, v[j] * up);
         }
-        if (n_ad > 0 && splits > 1) tc::cluster_sync();   // no CTA ends before its rows' words are read
     }
 }
 
@@ -1190,15 +1211,15 @@ struct Scratch {
 int64_t pad256(int64_t n) { return round_up(n, 256); }
 
 struct LowBytes {
-    int64_t t, parts, groups, wide, all;
+    int64_t t, parts, groups, power, all;
 };
 LowBytes low_bytes(const MultiLora& p, bool own_t) {
     LowBytes b;
     b.t = own_t ? pad256((int64_t)p.rows * p.rank * 4) : 0;
     b.parts = pad256((int64_t)p.rows * kPartSlots * low_parts(p.rank, p.dtype).cols * 2);
     b.groups = pad256(ceil_div(p.rows, 32) * 2 * (int64_t)sizeof(RowGroup));
-    b.wide = p.dtype == DT_F16 ? pad256((int64_t)p.rows * 16) : 0;
-    b.all = b.t + b.parts + b.groups + b.wide;
+    b.power = p.dtype == DT_F16 ? pad256(p.rows) : 0;
+    b.all = b.t + b.parts + b.groups + b.power;
     return b;
 }
 
@@ -1213,20 +1234,22 @@ constexpr int kTileRows = sizeof(T) == 4 ? 16 : 32;
 template <class T, bool TR>
 void shrink(const ShrinkArgs& a, bool tiles, cudaStream_t st) {
     ::bsml::count_launch();
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    auto go = [&](void (*kernel)(ShrinkArgs)) { BSML_CUDA(cudaLaunchKernelEx(&cfg, kernel, a)); };
     if (!tiles) {
-        shrink_rows_kernel<T, TR><<<dim3((unsigned)a.rows, (unsigned)ceil_div(a.rank, a.block)), kThreads, 0, st>>>(a);
+        cfg.gridDim = dim3((unsigned)a.rows, (unsigned)ceil_div(a.rank, a.block));
+        if (std::is_same<T, __half>::value) attr.val.clusterDim.y = cfg.gridDim.y;   // (at most 8: the row's power)
+        go(shrink_rows_kernel<T, TR>);
     } else {
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)a.splits;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(ceil_div(a.rows, kTileRows<T>) * a.splits));
-        cfg.blockDim = dim3(kThreads);
-        cfg.stream = st;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        auto go = [&](void (*kernel)(ShrinkArgs)) { BSML_CUDA(cudaLaunchKernelEx(&cfg, kernel, a)); };
+        attr.val.clusterDim.x = (unsigned)a.splits;
         if (a.rank <= 8) go(shrink_tile_kernel<T, TR, 1>);
         else if (a.rank <= 16) go(shrink_tile_kernel<T, TR, 2>);
         else if (a.rank <= 32) go(shrink_tile_kernel<T, TR, 4>);
@@ -1298,8 +1321,10 @@ struct Call {
         s.rng = p.rng;
         s.low = a.low;
         s.lp = low_parts(p.rank, p.dtype);
-        // few rows: a CTA for every 8 ranks, while they all run at once
-        s.block = (int64_t)p.rows * ceil_div(p.rank, 8) <= 592 ? 8 : (int)round_up(p.rank, 8);
+        // few rows: a CTA for every 8 ranks (fp16, a cluster a row: 8 CTAs at most), while they all run at once
+        s.block = (int64_t)p.rows * ceil_div(p.rank, 8) > 592          ? (int)round_up(p.rank, 8)
+                  : std::is_same<T, __half>::value && p.rank > 64 ? 16
+                                                                       : 8;
         s.splits = shrink_splits(ceil_div(p.rows, kTileRows<T>), a.width);
         const bool tiles = shrink_tiles<T>(p, a.width, mask.thr != 0);
         if (a.transposed) shrink<T, true>(s, tiles, st);
@@ -1356,7 +1381,7 @@ struct Call {
         low.t = t ? t : (float*)s.take(lb.t);
         low.parts = s.take(lb.parts);
         low.groups = (RowGroup*)s.take(lb.groups);
-        if (lb.wide) low.wide = (uint8_t*)s.take(lb.wide);
+        if (lb.power) low.power = (uint8_t*)s.take(lb.power);
     }
 
     void backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* h, void* dx, int64_t lddx,

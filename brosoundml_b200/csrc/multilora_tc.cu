@@ -76,7 +76,7 @@ struct PArgs {
     uint32_t idesc;              // without N
     const int* ids;
     const RowGroup* groups;
-    const uint8_t* wide;
+    const uint8_t* power;
     const float* t;
     const void* Q;               // as the caller has it
     int part_cols;               // of one slot
@@ -106,33 +106,25 @@ struct TileRows {
 // its use, so that nothing waits for it between two tiles.
 struct RawRows {
     int4 slot;              // and `rows`
-    uint4 rest;
+    uint2 rest;
 };
 __device__ __forceinline__ RawRows load_rows(const PArgs& a, int m0, int lane) {
-    RawRows r = {make_int4(-1, -1, -1, 0), make_uint4(0, 0, 0, 0)};
+    RawRows r = {make_int4(-1, -1, -1, 0), make_uint2(0, 0)};
     if (lane * 16 < a.np && m0 + lane * 16 < a.rows) {
         const int4* p = reinterpret_cast<const int4*>(a.groups + m0 / 16 + lane);
         r.slot = p[0];
-        r.rest = *reinterpret_cast<const uint4*>(p + 1);
+        r.rest = *reinterpret_cast<const uint2*>(p + 1);
     }
     return r;
 }
-template <bool WIDE, int G>
-__device__ __forceinline__ TileRows tile_rows(const PArgs& a, const RawRows& raw, int m0, int lane) {
+template <int G>
+__device__ __forceinline__ TileRows tile_rows(const RawRows& raw) {
     static_assert(kPartSlots == 3, "RowGroup in two vectors");
     const uint32_t all = 0xffffffffu;
     TileRows t;
     t.slot[0] = raw.slot.x; t.slot[1] = raw.slot.y; t.slot[2] = raw.slot.z;
     t.rows = (uint32_t)raw.slot.w;
     uint32_t many = raw.rest.x, without = raw.rest.y;
-    if (WIDE && __any_sync(all, raw.rest.z != 0))   // rows whose numbers do not fit their parts
-        for (int i = 0; i * 32 < a.np; ++i) {
-            const int m = m0 + i * 32 + lane;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (m < a.rows) w = *reinterpret_cast<const uint4*>(a.wide + (int64_t)m * 16);
-            const uint32_t bits = __ballot_sync(all, (w.x | w.y | w.z | w.w) != 0);
-            if (lane >> 1 == i) many |= lane & 1 ? bits >> 16 : bits & 0xFFFFu;
-        }
     if (G == 32) {
         many |= __shfl_xor_sync(all, many, 1);
         without |= __shfl_xor_sync(all, without, 1);
@@ -154,8 +146,28 @@ __device__ __forceinline__ TileRows tile_rows(const PArgs& a, const RawRows& raw
 
 // Whether the group's low-rank product is the MMAs' work.
 __device__ __forceinline__ bool by_mma(int gid) { return gid >= 0 || gid == kMixed; }
-// Whether that product has an accumulator of its own where there is no dropout.
-__device__ __forceinline__ bool apart(int gid) { return gid == kMixed; }
+// Whether that product has an accumulator of its own where there is no dropout. (fp16's always: it is in the
+// powers of two of its rows.)
+template <class T>
+__device__ __forceinline__ bool apart(int gid) {
+    return gid == kMixed || (std::is_same<T, __half>::value && gid >= 0);
+}
+
+// The powers of a lane's row (lane & 15) in N groups of 16, every second one from `g`, a byte each.
+template <int N>
+__device__ __forceinline__ uint64_t load_powers(const PArgs& a, int m0, int g, int lane) {
+    uint64_t p = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (g + 2 * i) * 16 + (lane & 15);
+        if (c < a.np && m0 + c < a.rows) p |= (uint64_t)a.power[m0 + c] << (8 * i);
+    }
+    return p;
+}
+// Number j of 16 columns (rows) times the power of its row: `power` is that of this lane's row.
+__device__ __forceinline__ uint32_t times_power(uint32_t v, uint32_t power, int j) {
+    return __float_as_uint(__uint_as_float(v) * __uint_as_float((__shfl_sync(0xffffffffu, power, j) & 0xFFu) << 23));
+}
 
 // A run of groups of one adapter in one slot: what the issuing threads go through. first: no
 // lower slot has an adapter in these groups; own: they are apart().
@@ -169,7 +181,7 @@ struct Run {
 typedef Run Runs[kPartSlots * kMaxGroups];
 // The tile's runs, by slot, then column; returns how many. By a whole warp: lane (slot k, group
 // g), because one thread's way through 24 places takes longer than the K steps that wait for it.
-template <int G>
+template <class T, int G>
 __device__ __forceinline__ int find_runs(Runs& out, const TileRows& rows, int groups, int lane) {
     const uint32_t all = 0xffffffffu;
     const int k = lane / kMaxGroups, g = lane % kMaxGroups;
@@ -182,7 +194,7 @@ __device__ __forceinline__ int find_runs(Runs& out, const TileRows& rows, int gr
     const uint32_t has = __ballot_sync(all, ad >= 0);
     int low = 0;
     for (int i = 0; i < kPartSlots - 1; ++i) low |= i < k ? has >> (i * kMaxGroups + g) & 1 : 0;
-    const int own = apart(__shfl_sync(all, rows.gid, g * (G / 16)));
+    const int own = apart<T>(__shfl_sync(all, rows.gid, g * (G / 16)));
     const int kind = low | own << 1, ad_before = __shfl_up_sync(all, ad, 1), kind_before = __shfl_up_sync(all, kind, 1);
     const bool start = ad >= 0 && (g == 0 || ad != ad_before || kind != kind_before);
     const uint32_t starts = __ballot_sync(all, start);
@@ -483,7 +495,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
     project_pair_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
                         const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mT,
                         const __grid_constant__ PArgs a) {
-    constexpr bool WIDE = std::is_same<T, __half>::value, F32 = sizeof(T) == 4;
+    constexpr bool F16 = std::is_same<T, __half>::value, F32 = sizeof(T) == 4;
     constexpr int B = kSums<T, DROP>;                // sums in TMEM
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
@@ -559,8 +571,8 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                 raw = load_rows(a, m0, lane);
                 dep = true;
             }
-            const TileRows rows = tile_rows<WIDE, 32>(a, raw, m0, lane);
-            const int n_runs = find_runs<32>(runs[0], rows, groups, lane);
+            const TileRows rows = tile_rows<32>(raw);
+            const int n_runs = find_runs<T, 32>(runs[0], rows, groups, lane);
             if (leader)
                 for (int i = 0; ok && i < n_runs; ++i) {
                     const Run u = runs[0][i];
@@ -624,9 +636,9 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                     raw = load_rows(a, m0, lane);
                     dep = true;
                 }
-                const TileRows rows = tile_rows<WIDE, 32>(a, raw, m0, lane);
-                const int n_runs = find_runs<32>(runs[1], rows, groups, lane);
-                const bool own = !DROP && __any_sync(0xffffffffu, apart(rows.gid));
+                const TileRows rows = tile_rows<32>(raw);
+                const int n_runs = find_runs<T, 32>(runs[1], rows, groups, lane);
+                const bool own = !DROP && __any_sync(0xffffffffu, apart<T>(rows.gid));
                 if (leader && ok) {
                     if (own) ok = vacant(buf ^ 1);
                     for (int i = 0; ok && i < n_runs; ++i) {
@@ -676,10 +688,10 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
         for (int tile = pair; tile < n_tiles; tile += pairs) {
             const TilePos at = tile_pos(a, tile);
             const int m0 = at.m * a.np, f = at.f * 256 + (int)rank * 128 + q * 32 + lane;
-            const TileRows rows = tile_rows<WIDE, 32>(a, load_rows(a, m0, lane), m0, lane);
+            const TileRows rows = tile_rows<32>(load_rows(a, m0, lane));
             const float bias = a.bias && f < a.feats ? to_f(((const T*)a.bias)[f]) : 0.f;
             const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
-            const bool own = !DROP && __any_sync(0xffffffffu, apart(rows.gid));
+            const bool own = !DROP && __any_sync(0xffffffffu, apart<T>(rows.gid));
             // groups whose low-rank product is not finite, and their rows once more, with the shared
             // sums at `column`
             uint32_t bad = 0;
@@ -744,7 +756,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                     if (g * 16 >= a.np) break;
                     const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
                     keep[i] = keep_of(g, gid);
-                    if (!(DROP ? by_mma(gid) : apart(gid))) continue;
+                    if (!(DROP ? by_mma(gid) : apart<T>(gid))) continue;
                     uint32_t x[8];
                     if (gid == kMixed) {
                         bool b = false;
@@ -795,6 +807,9 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                         const int g = h + HG * i;
                         turn(g * 16 < a.np ? keep_of(g, __shfl_sync(0xffffffffu, rows.gid, g & 31)) : 0u);
                     }
+                static_assert(HG == 2, "load_powers");
+                uint64_t powers = 0;
+                if (F16 && (DROP || own)) powers = load_powers<8>(a, m0, h, lane);
                 const int buf = u.next<B>();
                 ok = wait_sum(buf) && (!own || wait_sum(buf ^ 1));
                 if (!ok) break;
@@ -817,15 +832,20 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
 #pragma unroll 1
                     for (int g = h; g * 16 < a.np; g += HG) {
                         const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
-                        if (!apart(gid)) continue;
-                        sums_of(g, true);
-                        if (broken()) {
-                            bad |= 1u << g;
-                            continue;
-                        }
+                        if (apart<T>(gid)) {
+                            sums_of(g, true);
+                            if (F16)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(x[j]) + __uint_as_float(y[j]);
-                        tc::tmem_st16(xcol + (uint32_t)(g * 16), v);
+                                for (int j = 0; j < 16; ++j) y[j] = times_power(y[j], (uint32_t)powers, j);
+                            if (gid == kMixed && broken()) {
+                                bad |= 1u << g;
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(x[j]) + __uint_as_float(y[j]);
+                                tc::tmem_st16(xcol + (uint32_t)(g * 16), v);
+                            }
+                        }
+                        if (F16) powers >>= 8;
                     }
                     release(buf ^ 1);
                 }
@@ -836,6 +856,11 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                     sums_of(g, low);
                     const uint32_t keep = DROP ? kept[0] & 0xFFFFu : 0xFFFFu;
                     if (DROP) turn(0);
+                    if (DROP && F16) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = times_power(y[j], (uint32_t)powers, j);
+                        powers >>= 8;
+                    }
                     if (low && gid == kMixed && broken()) bad |= 1u << g;
                     if (bad >> g & 1) continue;
 #pragma unroll
@@ -869,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     project_split_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
                          const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mT,
                          const __grid_constant__ PArgs a) {
-    constexpr bool WIDE = std::is_same<T, __half>::value;
+    constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf;
@@ -946,8 +971,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tc::grid_dependency_wait();
         if (split == 0) {
-            const TileRows rows = tile_rows<WIDE, 16>(a, load_rows(a, m0, lane), m0, lane);
-            const int n_runs = find_runs<16>(runs[0], rows, groups, lane);
+            const TileRows rows = tile_rows<16>(load_rows(a, m0, lane));
+            const int n_runs = find_runs<T, 16>(runs[0], rows, groups, lane);
             if (leader)
                 for (int i = 0; ok && i < n_runs; ++i) {
                     const Run u = runs[0][i];
@@ -984,8 +1009,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tc::grid_dependency_wait();
         if (split == 0) {
-            const TileRows rows = tile_rows<WIDE, 16>(a, load_rows(a, m0, lane), m0, lane);
-            const int n_runs = find_runs<16>(runs[1], rows, groups, lane);
+            const TileRows rows = tile_rows<16>(load_rows(a, m0, lane));
+            const int n_runs = find_runs<T, 16>(runs[1], rows, groups, lane);
             if (leader)
                 for (int i = 0; ok && i < n_runs; ++i) {
                     const Run u = runs[1][i];
@@ -1032,7 +1057,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
         tc::grid_dependency_wait();
         const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
-        rows = tile_rows<WIDE, 16>(a, load_rows(a, m0, lane), m0, lane);
+        rows = tile_rows<16>(load_rows(a, m0, lane));
         bias = a.bias && f < a.feats ? to_f(((const T*)a.bias)[f]) : 0.f;
         if (a.splits > 1)   // the rows' t into L1, a load for every 32 bytes, all in flight
             for (int r = 0; r < a.rank; r += 8)
@@ -1064,6 +1089,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!(keep_bits(f >> 3, (uint32_t)m[j], key, a.drop.thr) >> (f & 7) & 1)) s[j] = 0.f;
                 low[i * 128] = make_float4(s[0], s[1], s[2], s[3]);
             }
+        uint32_t powers = 0;
+        if (F16 && split == 0) powers = (uint32_t)load_powers<4>(a, m0, h, lane);
         bool w = true;
         if (lane == 0) w = tc::mbar_wait(&accf, 0, err, tc::TC_ERR_WAIT_ACC);
         if (__shfl_sync(0xffffffffu, w ? 1 : 0, 0)) {
@@ -1086,12 +1113,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (ext) {
                     float e[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) e[j] = __uint_as_float(y[j]);
+                    for (int j = 0; j < 16; ++j) e[j] = __uint_as_float(F16 ? times_power(y[j], powers, j) : y[j]);
                     own_low<T, TR>(a, gid, m0 + g * 16, live, f, e);
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (keep >> j & 1) s[j] += e[j];
                 }
+                if (F16) powers >>= 8;
                 if (a.splits == 1) {   // nothing to join
                     finish_rows<T, TR>(a, rows, g, gid, m0 + g * 16, f, keep, bias, s);
                     continue;
@@ -1345,7 +1373,7 @@ void run(const ProjectTc& p, const Operands& o, cudaStream_t st) {
     }
     const LowParts lp = low_parts(p.rank, p.dtype);
     make_ext(a, lp, p.dtype == DT_F32 ? 3 : 1);
-    a.ids = p.ids; a.groups = p.low.groups; a.wide = p.low.wide; a.t = p.low.t;
+    a.ids = p.ids; a.groups = p.low.groups; a.power = p.low.power; a.t = p.low.t;
     a.Q = p.Q; a.bias = p.bias;
     a.part_cols = lp.cols;
     a.drop = p.drop; a.rng = p.rng; a.zero_padding = p.zero_padding;

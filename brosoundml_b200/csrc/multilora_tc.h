@@ -14,10 +14,9 @@ constexpr int kPartSlots = 3;
 struct alignas(32) RowGroup {
     int slot[kPartSlots];        // the adapter of each slot (LowParts), -1 for none
     uint32_t rows;               // bit j: row j is read and written (id >= -1); bit 16 + j: it is padding
-    uint32_t many;               // rows of later runs than there are slots, or whose numbers do not fit their parts
+    uint32_t many;               // rows of later runs than there are slots
     uint32_t without;            // live rows without an adapter
-    uint32_t check;              // 1: whether they fit stands in LowRank::wide
-    uint32_t pad;
+    uint32_t pad[2];
 };
 
 // The rank numbers of every row between the two low-rank products: `t` as they are, and
@@ -26,9 +25,8 @@ struct LowRank {
     float* t = nullptr;              // (rows, rank)
     void* parts = nullptr;           // (rows, kPartSlots * cols of low_parts(rank, dtype)), 16-bit
     RowGroup* groups = nullptr;      // (rows / 32 rounded up, 2)
-    // (rows, 16), fp16 only, where RowGroup::check says so: byte r / 8 is 1 where number r does not
-    // fit its parts
-    uint8_t* wide = nullptr;
+    // (rows), fp16 only: the parts are the row's numbers over the power of two of this biased exponent
+    uint8_t* power = nullptr;
 };
 
 // Layout of LowRank::parts. A row has kPartSlots pieces of `cols` columns; its numbers are in the
@@ -36,7 +34,9 @@ struct LowRank {
 // in a row with one adapter) among the runs that begin in, or reach into, its 32 rows (32 i ..
 // 32 i + 31); the parts of a row of a later run than kPartSlots are not used. In a piece: number r
 // of part i in column i * pitch + r, zero up to the pitch; the parts sum to the number. 16-bit
-// types hold two parts of their own type, fp32 three bf16 parts (24 bits).
+// types hold two parts of their own type, fp32 three bf16 parts (24 bits). fp16's are of the row's numbers over
+// a power of two that brings the largest to 2^14 .. 2^15: as they are, a number beyond 65504 would have no
+// parts, and one below 1/8 (gradients are below 1e-4) fewer than 22 bits.
 struct LowParts {
     int n = 0, pitch = 0, cols = 0;
 };

@@ -409,8 +409,7 @@ int bsml_convlora_load(bsml_convlora* l, const char* path);
  * h (rows, rank, float). Rows do not mix: a NaN or infinity in one row or one
  * adapter stays in the rows of its own. Sums are kept in fp32 and rounded once to
  * the dtype; the tensor cores take h (and the backward's g) as two numbers of a 16-bit
- * dtype (off by 2^-17 in bf16; in fp16 by 2^-22, or 2^-25 absolute below 1/8, which an
- * output feels where it is itself near fp16's smallest numbers, or B's far above 1) and
+ * dtype (off by 2^-17 in bf16, by 2^-22, or 2^-39 of the row's largest number, in fp16) and
  * as three bf16 numbers in fp32. rank is 1..BSML_MULTILORA_MAX_RANK, cin and cout at most 2^20.
  * Dropout of the adapters' input (not of the shared projection's) has probability
  * p in steps of 2^-16; its mask is bsml_dropout_forward's of a (rows, cin) tensor,

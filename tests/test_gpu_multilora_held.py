@@ -66,7 +66,7 @@ def test_a_refused_call_leaves_nothing_behind():
         assert torch.equal(got[k], want[k]), k
 
 
-@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("rank", [1, 4, 12])
 @pytest.mark.parametrize("rows", [2, 1500])
 def test_the_smallest_adapter_at_its_buffers_end(dtype, rank, rows):
@@ -190,3 +190,44 @@ def test_no_numbers_hold_a_call_up(dtype, where):
         assert bool(torch.isfinite(g).all())
         tol = torch.finfo(c["x"].dtype).eps * w.abs() + 2 * (W + 10) * 2.0**-23 * 4 * W**0.5
         assert bool(((w - g).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("shape", [(40, 1032, 200, 8, 4, "scattered"), (16, 1024, 320, 100, 3, "runs"), (900, 640, 1030, 16, 3, "runs"),
+                                   (3000, 640, 1700, 40, 4, "short"), (600, 600, 320, 24, 2, "runs")],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("p", [0.0, 0.25])
+@pytest.mark.parametrize("rows,adapters", [(1e-5, 300.0), (2.0**-20, 1000.0), (1.0, 1e-4)])
+def test_small_numbers_between_the_products_fp16(shape, p, rows, adapters):
+    """h and g of any size keep their relative accuracy beside fp16 operands: where they are far below fp16's
+    normal numbers and the adapters' entries above 1, the outputs are within the bounds all the same."""
+    c = _make("fp16", *shape, seed=7)
+    for k in ("x", "dy"):
+        c[k] *= rows
+    c["A"] = (c["A"].float() * adapters).half()
+    c["B"] = (c["B"].float() * adapters / 8).half()
+    c["W"] *= 2.0**-6
+    c["scale"] *= 2.0**-10 if adapters > 1 else 1.0
+    want = _expect(c, p=p, bias=False)
+    assert float(want["h"][0].abs().max()) < (0.25 if adapters > 1 else 2.0**-6)
+    got = _run(c, p=p, bias=False)
+    assert all(bool(torch.isfinite(got[k]).all()) for k in ("y", "dx"))
+    _agree(got, {k: want[k] for k in ("y", "h", "dx")})
+
+
+@pytest.mark.parametrize("M", [24, 1500])
+def test_rows_of_very_different_sizes_fp16(M):
+    """Rows whose numbers differ by 2^60 among neighbours, and numbers of a row by 2^16."""
+    c = _make("fp16", M, 640, 320, 12, 3, "runs", seed=9)
+    c["scale"] = torch.tensor([2.0**-40, 1.0, 2.0**20], device="cuda")
+    c["A"][:, ::3] *= 2.0**-10
+    c["x"] *= 2.0**-12
+    c["x"][::2] *= 2.0**-4
+    c["B"] *= 2.0**-6
+    c["dy"] *= 2.0**-10
+    want = _expect(c, bias=False)
+    got = _run(c, bias=False)
+    # (what is beyond fp16's range in the outputs is infinite there)
+    for k in ("y", "h", "dx"):
+        fits = want[k][0].abs() < 65000
+        assert bool(torch.isfinite(got[k].cpu()[fits]).all())
+        assert ref.worst(got[k].cpu()[fits], tuple(v[fits] for v in want[k])) <= 1.0, k
