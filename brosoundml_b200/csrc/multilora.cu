@@ -27,11 +27,11 @@ constexpr int kThreads = 256;
 constexpr int kMaxRank = 128;
 
 // ── h and g: rows times an adapter's thin matrix
-// A number as the parts of LowParts: two of its 16-bit type, or three bf16 ones. Each part is
-// the rounded remainder of those before it, a number that is not finite has no remainder. Two parts
-// and not the fp32 number, because the product then needs no accumulator of another type beside
-// the shared projection's: bf16 keeps 16 bits (an output's rounding is 8), fp16 (v: times its row's power of two)
-// 22, or steps of 2^-39 of the row's largest number.
+// A number as the parts of LowParts: three bf16 numbers, or two fp16 ones. Each part is the rounded
+// remainder of those before it, a number that is not finite has no remainder. bf16's three hold an fp32
+// number whole (below 2^-110 less); fp16's two, of `v` over its row's power of two, 22 bits or steps of
+// 2^-39 of the row's largest number: a third would add 2^-23 of it, where h itself is off by more after its
+// sum, and an output by 2^-11.
 template <class T>
 __device__ __forceinline__ void put_parts(uint16_t* row, const LowParts& lp, int r, float v) {
     if constexpr (!std::is_same<T, __half>::value) {

@@ -55,7 +55,7 @@ constexpr int kPromote = 8;           // K steps of 64 in one fp32 accumulator (
 constexpr int kMaxExt = 12;
 
 // One TMA stage of the low-rank K steps: 64 ranks of Q plane `plane` from rank `rank0`, 64
-// columns of the parts from `col0`, and the 16-rank steps that pair them.
+// columns of the parts from `col0`, and the steps of 16 ranks that pair them (4 at most).
 struct ExtStage {
     int8_t plane, n;
     int16_t rank0, col0;
@@ -1331,31 +1331,30 @@ void launch(K kernel, int grid, int threads, int cluster, int smem, cudaStream_t
     BSML_CUDA(cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], a));
 }
 
-// The plane products of one low-rank stage, smallest first.
+// The plane products of the low-rank stages, smallest first: a stage is 64 ranks of a plane of Q and 64 columns of
+// the parts, which hold several parts where the ranks are few.
 void make_ext(PArgs& a, const LowParts& lp, int planes) {
-    const int blocks = (int)ceil_div(a.rank, 64), steps = (int)ceil_div(std::min(a.rank, 64), 16);
+    const int blocks = (int)ceil_div(a.rank, 64);
     a.n_ext = 0;
-    const bool packed = lp.cols <= 64;   // every part in one 64-column block
     for (int q = planes - 1; q >= 0; --q)
-        for (int b = 0; b < blocks; ++b) {
-            const int parts = planes == 1 ? lp.n : lp.n - q;   // fp32: plane q meets parts 0 .. 2 - q
-            for (int i = parts - 1; i >= 0; --i) {
-                if (!packed || i == parts - 1) {
-                    ExtStage& x = a.ext[a.n_ext++];
-                    x = ExtStage{};
-                    x.plane = (int8_t)q;
-                    x.rank0 = (int16_t)(b * 64);
-                    x.col0 = (int16_t)(packed ? 0 : i * lp.pitch + b * 64);
+        for (int b = 0; b < blocks; ++b)
+            for (int i = (planes == 1 ? lp.n : lp.n - q) - 1; i >= 0; --i) {   // fp32: plane q meets parts 0 .. 2 - q
+                const int col = i * lp.pitch + b * 64, col0 = col / 64 * 64;
+                ExtStage* x = a.n_ext ? &a.ext[a.n_ext - 1] : nullptr;
+                if (!x || x->plane != q || x->rank0 != b * 64 || x->col0 != col0) {
+                    x = &a.ext[a.n_ext++];
+                    *x = ExtStage{};
+                    x->plane = (int8_t)q;
+                    x->rank0 = (int16_t)(b * 64);
+                    x->col0 = (int16_t)col0;
                 }
-                ExtStage& x = a.ext[a.n_ext - 1];
-                const int here = packed ? steps : (int)ceil_div(std::min(a.rank - b * 64, 64), 16);
-                for (int s = 0; s < here; ++s) {
-                    x.a[x.n] = (int8_t)s;
-                    x.b[x.n] = (int8_t)(s + (packed ? i * lp.pitch / 16 : 0));
-                    ++x.n;
+                const int steps = (int)ceil_div(std::min(a.rank - b * 64, 64), 16);
+                for (int s = 0; s < steps; ++s) {
+                    x->a[x->n] = (int8_t)s;
+                    x->b[x->n] = (int8_t)(s + (col - col0) / 16);
+                    ++x->n;
                 }
             }
-        }
 }
 
 template <class T, bool TR, bool DROP>
@@ -1458,10 +1457,9 @@ void run_type(const ProjectTc& p, const Operands& o, cudaStream_t st) {
 
 LowParts low_parts(int rank, int dtype) {
     LowParts l;
-    l.n = dtype == DT_F32 ? 3 : 2;
-    const int small = (int)round_up(rank, 16);
-    l.pitch = l.n * small <= 64 ? small : (int)round_up(rank, 64);
-    l.cols = (int)std::max<int64_t>(64, (int64_t)l.n * l.pitch);
+    l.n = dtype == DT_F16 ? 2 : 3;
+    l.pitch = rank <= 16 ? 16 : rank <= 32 ? 32 : (int)round_up(rank, 64);   // no part over a stage's end
+    l.cols = (int)round_up(l.n * l.pitch, 64);
     return l;
 }
 

@@ -33,8 +33,8 @@ struct LowRank {
 // piece of its slot, the other pieces are zero. The slot is the ordinal of the row's run (rows
 // in a row with one adapter) among the runs that begin in, or reach into, its 32 rows (32 i ..
 // 32 i + 31); the parts of a row of a later run than kPartSlots are not used. In a piece: number r
-// of part i in column i * pitch + r, zero up to the pitch; the parts sum to the number. 16-bit
-// types hold two parts of their own type, fp32 three bf16 parts (24 bits). fp16's are of the row's numbers over
+// of part i in column i * pitch + r, zero up to the pitch; the parts sum to the number. bf16
+// and fp32 hold three bf16 parts (24 bits), fp16 two of its own (22). fp16's are of the row's numbers over
 // a power of two that brings the largest to 2^14 .. 2^15: as they are, a number beyond 65504 would have no
 // parts, and one below 1/8 (gradients are below 1e-4) fewer than 22 bits.
 struct LowParts {

@@ -408,9 +408,9 @@ int bsml_convlora_load(bsml_convlora* l, const char* path);
  * cout) with row stride ldy, all of one dtype; scale (adapters, float) or NULL for 1;
  * h (rows, rank, float). Rows do not mix: a NaN or infinity in one row or one
  * adapter stays in the rows of its own. Sums are kept in fp32 and rounded once to
- * the dtype; the tensor cores take h (and the backward's g) as two numbers of a 16-bit
- * dtype (off by 2^-17 in bf16, by 2^-22, or 2^-39 of the row's largest number, in fp16) and
- * as three bf16 numbers in fp32. rank is 1..BSML_MULTILORA_MAX_RANK, cin and cout at most 2^20.
+ * the dtype; the tensor cores take h (and the backward's g) as three bf16 numbers, which
+ * hold an fp32 number whole, and beside fp16 operands as two fp16 ones (off by 2^-22, or
+ * 2^-39 of the row's largest number). rank is 1..BSML_MULTILORA_MAX_RANK, cin and cout at most 2^20.
  * Dropout of the adapters' input (not of the shared projection's) has probability
  * p in steps of 2^-16; its mask is bsml_dropout_forward's of a (rows, cin) tensor,
  * never stored: the backward makes it again from rng = {seed, offset} (two

@@ -231,3 +231,35 @@ def test_rows_of_very_different_sizes_fp16(M):
         fits = want[k][0].abs() < 65000
         assert bool(torch.isfinite(got[k].cpu()[fits]).all())
         assert ref.worst(got[k].cpu()[fits], tuple(v[fits] for v in want[k])) <= 1.0, k
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rank", [2, 8, 20, 40])
+@pytest.mark.parametrize("M,length", [(40, 1), (40, 16), (700, 13), (3000, 300), (3000, 9)])
+def test_numbers_between_the_products_are_whole(dtype, rank, M, length):
+    """Products that cancel: ranks in pairs, h = s (a, b, ..) times B = (b, -a, ..), and g = s (b, -a, ..) times
+    A = (a, b, ..), with s of 24 bits. What is left is what the numbers between the products lost: nothing of
+    fp32's 24 bits, 2^-22 beside fp16 operands, and 2^-23 for each of the sum's additions (an MMA for every 16
+    ranks and part or plane product, 6 at most, the rows' two and the epilogue's two)."""
+    L, t = _lora(), TYPES[dtype]
+    K, N, nA = 640, 1700 if M > 1000 else 264, 16
+    g = torch.Generator().manual_seed(rank + M)
+    a = (torch.randn(nA, rank, generator=g)).to(t)
+    b = torch.empty_like(a)
+    b[:, 0::2], b[:, 1::2] = a[:, 1::2], -a[:, 0::2]
+    A, B = a[:, :, None].expand(-1, -1, K).contiguous().cuda(), b[:, None, :].expand(-1, N, -1).contiguous().cuda()
+    scale = (torch.rand(nA, generator=g) + 0.5).cuda()
+    ids = (torch.arange(M) // length % nA).int().cuda()
+    x, dy = torch.zeros(M, K, dtype=t, device="cuda"), torch.zeros(M, N, dtype=t, device="cuda")
+    x[torch.arange(M), torch.arange(M) % K] = 1
+    dy[torch.arange(M), torch.arange(M) % N] = 1
+    W = torch.zeros(N, K, dtype=t, device="cuda")
+    h = torch.empty(M, rank, device="cuda")
+    y = L.multi_lora_forward(x, W, A, B, ids, scale=scale, h=h)
+    dx = L.multi_lora_backward(dy, x, W, A, B, ids, h, scale=scale, want_adapters=False)["dx"]
+    sizes = (scale.double() * (a.double() * b.double()).abs().sum(1).cuda())[ids.long()]
+    adds = 6 * (-(-rank // 16)) + 4
+    bound = ((2.0**-22 if dtype == "fp16" else 0.0) + adds * 2.0**-23) * sizes + (2.0**-25 if dtype == "fp16" else 0.0)
+    for k, v in (("y", y), ("dx", dx)):
+        worst = float((v.double().abs().amax(1) / bound).max())
+        assert worst <= 1.0, f"{k}: {worst:.3g} times its bound"
