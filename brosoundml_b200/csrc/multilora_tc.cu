@@ -15,8 +15,11 @@
 // fp32 runs as bf16 planes: an fp32 number is the sum of three bf16 numbers, and the six plane
 // products of significance 2^-16 and above are six passes of the same K loop, the smallest
 // first: the accumulator's truncations are relative to its value, which stays small until the
-// last pass. In the pair kernel the sums also leave the accumulator every kPromote steps for
-// registers, where fp32 adds round to nearest.
+// last pass.
+// Every MMA truncates the accumulator's sum, always towards zero: positive fp16 numbers lose 6e-9 of
+// their sum a column (measured: 4e-4 over 65536 columns; fp32's planes 8e-4 over 131072). So long sums leave
+// the accumulator for registers, where fp32 adds round to nearest: fp32's every 512 columns of a pass
+// (9e-7), 16-bit types' every 4096 (2e-5, 1/20 of an fp16 output's rounding).
 #include "multilora_tc.h"
 
 #include <cuda_bf16.h>
@@ -51,7 +54,9 @@ constexpr int kTileA = 16384;         // 128 features x 128 bytes of K
 constexpr int kMaxStages = 12;
 constexpr int kThreads = 320;         // split kernel: TMA warp, MMA warp, 8 epilogue warps
 constexpr int kMaxTerms = 6;
-constexpr int kPromote = 8;           // K steps of 64 in one fp32 accumulator (pair kernel)
+// K steps of 64 in one accumulator, where sums are longer
+template <class T>
+constexpr int kPromote = sizeof(T) == 4 ? 8 : 64;
 constexpr int kMaxExt = 12;
 
 // One TMA stage of the low-rank K steps: 64 ranks of Q plane `plane` from rank `rank0`, 64
@@ -153,13 +158,13 @@ __device__ __forceinline__ bool apart(int gid) {
     return gid == kMixed || (std::is_same<T, __half>::value && gid >= 0);
 }
 
-// The powers of a lane's row (lane & 15) in N groups of 16, every second one from `g`, a byte each.
-template <int N>
+// The powers of a lane's row (lane & 15) in N groups of 16, every STEP-th one from `g`, a byte each.
+template <int N, int STEP>
 __device__ __forceinline__ uint64_t load_powers(const PArgs& a, int m0, int g, int lane) {
     uint64_t p = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int c = (g + 2 * i) * 16 + (lane & 15);
+        const int c = (g + STEP * i) * 16 + (lane & 15);
         if (c < a.np && m0 + c < a.rows) p |= (uint64_t)a.power[m0 + c] << (8 * i);
     }
     return p;
@@ -442,18 +447,17 @@ struct Ring {
 };
 
 // Accumulators of a pair, and columns of its tile. TMEM's 512 columns hold two sums, or with dropout
-// (whose low-rank product has an accumulator of its own) one sum and that. fp32's sums are many a
-// tile, so it has two beside that of the low-rank product. (16-bit with two of 160 columns: 244 us
-// where one of 256, its epilogue not hidden, takes 200: 8192 x 4096 x 4096, 16 ranks. L2 bounds
-// narrow tiles.)
-template <class T, bool DROP>
-constexpr int kSums = DROP && sizeof(T) == 2 ? 1 : 2;
-template <class T, bool DROP>
-constexpr int kMaxColumns = DROP && sizeof(T) == 4 ? 160 : 256;
-// Epilogue warps of a pair's CTA. fp32's running sums take 16 columns x groups registers a
+// (whose low-rank product has an accumulator of its own) one sum and that. Where a tile has many sums (LONG),
+// there are two beside that of the low-rank product. (16-bit with two of 160 columns: 244 us where one of
+// 256, its epilogue not hidden, takes 200: 8192 x 4096 x 4096, 16 ranks. L2 bounds narrow tiles.)
+template <bool DROP, bool LONG>
+constexpr int kSums = DROP && !LONG ? 1 : 2;
+template <bool DROP, bool LONG>
+constexpr int kMaxColumns = DROP && LONG ? 160 : 256;
+// Epilogue warps of a pair's CTA. Many sums run in 16 columns x groups registers a
 // thread: 16 warps of 64 sums (and at most 96 registers) hold 256 columns.
-template <class T>
-constexpr int kPairEpi = sizeof(T) == 4 ? 16 : 8;
+template <bool LONG>
+constexpr int kPairEpi = LONG ? 16 : 8;
 
 // A tile's sums go to the accumulators in turn, whose uses every role counts alike: `at` is the next one, bit i
 // of `uses` whether i was used an odd number of times. A tile with groups apart() also uses, for these, the one after its last
@@ -490,13 +494,13 @@ __device__ __forceinline__ TilePos tile_pos(const PArgs& a, int tile) {
 // Bound by the tensor pipe at 256 columns (about 560 cycles for 64 columns of K, of which 512 are
 // MMAs), by L2's operand rate below: 8192 x 4096 x 4096 bf16 187 us alone (1.47 PFLOP/s; the low-rank
 // steps of 16 ranks and 8 prompts add 3), 203 with dropout; 2048 x 2048 x 2048 fp32 106 us.
-template <class T, bool TR, bool DROP>
-__global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
+template <class T, bool TR, bool DROP, bool LONG>
+__global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
     project_pair_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
                         const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mT,
                         const __grid_constant__ PArgs a) {
-    constexpr bool F16 = std::is_same<T, __half>::value, F32 = sizeof(T) == 4;
-    constexpr int B = kSums<T, DROP>;                // sums in TMEM
+    constexpr bool F16 = std::is_same<T, __half>::value;
+    constexpr int B = kSums<DROP, LONG>;             // sums in TMEM
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf[2], acce[2], mdone;
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
         }
         for (int s = 0; s < 2; ++s) {
             tc::mbar_init(&accf[s], 1);
-            tc::mbar_init(&acce[s], 2 * kPairEpi<T>);
+            tc::mbar_init(&acce[s], 2 * kPairEpi<LONG>);
         }
         tc::mbar_init(&mdone, 1);
         gave_up = tc::TC_OK;
@@ -537,8 +541,8 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
     const int n_tiles = a.n_ft * a.n_mt;
     const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
     const int steps = a.n_terms * a.kchunks;
-    // sums a tile: fp32 leaves the accumulator every kPromote steps
-    const int sums = F32 ? (steps + kPromote - 1) / kPromote : 1;
+    // sums a tile
+    const int sums = LONG ? (steps + kPromote<T> - 1) / kPromote<T> : 1;
 
     if (warp == 0) {
         // ── TMA producer (both CTAs, into their own shared memory; the even CTA's barrier
@@ -609,7 +613,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                     buf = u.next<B>();
                     if (leader && ok) {
                         const uint32_t idesc = idesc_n(a.idesc, a.np);
-                        const int first = F32 ? g * kPromote : 0, n = F32 ? min(steps - first, kPromote) : steps;
+                        const int n = LONG ? min(steps - g * kPromote<T>, kPromote<T>) : steps;
                         ok = vacant(buf);
                         for (int c = 0; ok && c < n; ++c) {
                             ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
         }
     } else {
         // ── epilogue: warp (q, h) has TMEM lanes 32q.. and every HG-th group of 16 rows
-        constexpr int HG = kPairEpi<T> / 4;
+        constexpr int HG = kPairEpi<LONG> / 4;
         tc::grid_dependency_wait();
         const int q = warp & 3, h = (warp - 2) >> 2;
         const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
@@ -722,8 +726,10 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                 if (lane == 0) tc::mbar_arrive_cluster(lead[i]);
                 u.used(i);
             };
-            if constexpr (F32) {
-                constexpr int NG = (kMaxColumns<T, DROP> / 16 + HG - 1) / HG;   // this warp's column groups
+            if constexpr (LONG) {
+                constexpr int NG = (kMaxColumns<DROP, LONG> / 16 + HG - 1) / HG;   // this warp's column groups
+                uint32_t powers = 0;
+                if (F16 && (DROP || own)) powers = (uint32_t)load_powers<NG, HG>(a, m0, h, lane);
                 float v[NG][16] = {};
                 uint32_t keep[NG];
                 int buf = 0;
@@ -778,8 +784,10 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                         tc::tmem_ld8_nowait(trow + (uint32_t)(lowc + g * 16 + o), x);
                         tc::tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
+                        for (int j = 0; j < 8; ++j) {
+                            if (F16) x[j] = times_power(x[j], powers >> 8 * i, o + j);
                             if (keep[i] >> (o + j) & 1) v[i][o + j] += __uint_as_float(x[j]);
+                        }
                     }
                 }
                 if (!bad) release(low);
@@ -809,7 +817,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
                     }
                 static_assert(HG == 2, "load_powers");
                 uint64_t powers = 0;
-                if (F16 && (DROP || own)) powers = load_powers<8>(a, m0, h, lane);
+                if (F16 && (DROP || own)) powers = load_powers<8, 2>(a, m0, h, lane);
                 const int buf = u.next<B>();
                 ok = wait_sum(buf) && (!own || wait_sum(buf ^ 1));
                 if (!ok) break;
@@ -889,7 +897,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<T>, 1)
 // reading W once: every SM has a TMA ring of its own share of K in flight. One token of 4096 x 4096
 // bf16 (34 MB) 13 us after a thin product of 5.7 that it overlaps; 64 tokens of 32 requests x 4096 x 8192
 // (81 MB) 25.
-template <class T, bool TR, bool DROP>
+template <class T, bool TR, bool DROP, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
     project_split_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
                          const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mT,
@@ -897,7 +905,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool F16 = std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf;
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf[2], acce[2], mdone;
     __shared__ uint32_t tslot;
     __shared__ int gave_up;
     __shared__ Runs runs[2];
@@ -913,6 +921,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int k_lo = split * a.kchunks / a.splits, k_n = (split + 1) * a.kchunks / a.splits - k_lo;
     const int steps = a.n_terms * k_n;
 
+    // one sum in TMEM, or two in turn, and the low-rank product
+    constexpr int kLow = LONG ? 256 : 128, kColumns = 2 * kLow;
+    const int sums = LONG ? (steps + kPromote<T> - 1) / kPromote<T> : 1;
     // The ring's barriers are this CTA's own: its first loads go out before the cluster meets. (A
     // few: the TMA unit takes more only at the pace of memory, and the others wait here.)
     const int head = min(min(steps, a.stages), 2);
@@ -921,7 +932,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&full[s], 1);
             tc::mbar_init(&empty[s], 1);
         }
-        tc::mbar_init(&accf, 1);
+        for (int s = 0; s < 2; ++s) {
+            tc::mbar_init(&accf[s], 1);
+            tc::mbar_init(&acce[s], kThreads / 32 - 2);
+        }
+        tc::mbar_init(&mdone, 1);
         gave_up = tc::TC_OK;
         tc::fence_barrier_init();
         tc::fence_async_shared();
@@ -932,14 +947,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     if (warp == 1) {
-        tc::tmem_alloc(&tslot, 256);
+        tc::tmem_alloc(&tslot, kColumns);
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
     __syncthreads();
     tc::cluster_sync();   // every CTA of the cluster runs before any writes to its shared memory
     tc::tc_fence_after();
-    const uint32_t tbase = tslot, de = tbase + 128;   // the shared sum; the low-rank product's
+    const uint32_t tbase = tslot, de = tbase + kLow;
 
     // epilogue state that outlives the cluster barrier
     const int q = warp & 3, h = (warp - 2) >> 2;
@@ -993,17 +1008,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         if (leader) {
             const uint32_t idesc = idesc_n(a.idesc, a.np);
-            for (int c = 0; ok && c < steps; ++c) {
-                ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
-                if (!ok) break;
-                tc::tc_fence_after();
-                const uint32_t base = tc::smem_u32(smem + r.slot * stage_bytes);
+            for (int s = 0; ok && s < sums; ++s) {
+                const int n = LONG ? min(steps - s * kPromote<T>, kPromote<T>) : steps;
+                const uint32_t d = tbase + (uint32_t)((s & 1) * 128);
+                if (LONG && s >= 2) ok = tc::mbar_wait(&acce[s & 1], (s / 2 - 1) & 1, err, tc::TC_ERR_WAIT_ACC);
+                for (int c = 0; ok && c < n; ++c) {
+                    ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t base = tc::smem_u32(smem + r.slot * stage_bytes);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma<false>(tbase, desc_a<TR>(base, k), tc::desc_kmajor_sw128(base + kTileA + k * 32), idesc,
-                               (c | k) != 0);
-                commit<false>(&empty[r.slot]);
-                r.next(a.stages);
+                    for (int k = 0; k < 4; ++k)
+                        mma<false>(d, desc_a<TR>(base, k), tc::desc_kmajor_sw128(base + kTileA + k * 32), idesc,
+                                   (c | k) != 0);
+                    commit<false>(&empty[r.slot]);
+                    r.next(a.stages);
+                }
+                if (ok && s + 1 < sums) commit<false>(&accf[s & 1]);
             }
         }
         __syncwarp();
@@ -1031,8 +1052,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
         }
         if (leader) {   // also after an error: whatever was issued completes
-            commit<false>(&accf);
-            tc::mbar_wait(&accf, 0, nullptr, tc::TC_ERR_DRAIN);
+            if (ok) commit<false>(&accf[(sums - 1) & 1]);
+            commit<false>(&mdone);
+            tc::mbar_wait(&mdone, 0, nullptr, tc::TC_ERR_DRAIN);
         }
     } else {
         // The adapters of this CTA's rows, lane l those of columns l, l + 32, .., and the rows of Q
@@ -1055,6 +1077,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int ad = ad_of(c + j);
                     if (ad >= 0 && f < a.feats) tc::prefetch_l2((const T*)a.Q + ((int64_t)ad * a.feats + f) * a.rank);
                 }
+        // Many sums as they come: the first half of them before anything that waits for the kernel before, the
+        // others but the last one after it.
+        constexpr int NG = 4;   // this warp's groups, at most
+        const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
+        float acc[LONG ? NG : 1][16] = {};
+        auto wait_sum = [&](int s) {
+            bool w = true;
+            if (lane == 0) w = tc::mbar_wait(&accf[s & 1], (s >> 1) & 1, err, tc::TC_ERR_WAIT_ACC);
+            const bool got = __shfl_sync(0xffffffffu, w ? 1 : 0, 0) != 0;
+            tc::tc_fence_after();
+            return got;
+        };
+        bool ok = true;
+        auto take_sums = [&](int first, int end) {
+            if constexpr (LONG) {
+#pragma unroll 1
+                for (int s = first; ok && s < end; ++s) {
+                    ok = wait_sum(s);
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        const int g = h + 2 * i;
+                        if (g >= groups) break;
+                        uint32_t x[16];
+                        tc::tmem_ld16_nowait(trow + (uint32_t)((s & 1) * 128 + g * 16), x);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) acc[i][j] += __uint_as_float(x[j]);
+                    }
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&acce[s & 1]);
+                }
+            }
+        };
+        take_sums(0, sums / 2);
         tc::grid_dependency_wait();
         const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
         rows = tile_rows<16>(load_rows(a, m0, lane));
@@ -1090,26 +1148,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 low[i * 128] = make_float4(s[0], s[1], s[2], s[3]);
             }
         uint32_t powers = 0;
-        if (F16 && split == 0) powers = (uint32_t)load_powers<4>(a, m0, h, lane);
-        bool w = true;
-        if (lane == 0) w = tc::mbar_wait(&accf, 0, err, tc::TC_ERR_WAIT_ACC);
-        if (__shfl_sync(0xffffffffu, w ? 1 : 0, 0)) {
-            tc::tc_fence_after();
-            const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
+        if (F16 && split == 0) powers = (uint32_t)load_powers<NG, 2>(a, m0, h, lane);
+        take_sums(sums / 2, sums - 1);
+        if (ok && wait_sum(sums - 1)) {
+            const int last = LONG ? ((sums - 1) & 1) * 128 : 0;
             const uint32_t mine = tc::smem_u32(recv) + (uint32_t)((split * a.qpo * 128 + q * 32 + lane) * 16);
-            for (int g = h; g < groups; g += 2) {
+#pragma unroll(LONG ? NG : 1)
+            for (int i = 0; i < NG; ++i) {
+                const int g = h + 2 * i;
+                if (g >= groups) break;
                 uint32_t v[16], y[16];
                 const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
                 const uint32_t live = __shfl_sync(0xffffffffu, rows.rows, g) & 0xFFFFu;
                 const bool ext = split == 0 && by_mma(gid);
-                tc::tmem_ld16_nowait(trow + (uint32_t)(g * 16), v);
-                if (ext) tc::tmem_ld16_nowait(trow + (uint32_t)(128 + g * 16), y);
+                tc::tmem_ld16_nowait(trow + (uint32_t)(last + g * 16), v);
+                if (ext) tc::tmem_ld16_nowait(trow + (uint32_t)(kLow + g * 16), y);
                 tc::tmem_wait_ld();
                 uint32_t keep = 0xFFFFu;
                 if (DROP && (ext || (a.splits == 1 && gid == kMany))) keep = keep_columns(a, m0 + g * 16, f, lane, key);
                 float s[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(v[j]);
+                for (int j = 0; j < 16; ++j) s[j] = (LONG ? acc[LONG ? i : 0][j] : 0.f) + __uint_as_float(v[j]);
                 if (ext) {
                     float e[16];
 #pragma unroll
@@ -1142,7 +1201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::cluster_sync();
     tc::tc_fence_after();
     if (threadIdx.x == 0) report(gave_up);
-    if (warp == 1) tc::tmem_dealloc(tbase, 256);
+    if (warp == 1) tc::tmem_dealloc(tbase, kColumns);
     if (warp >= 2 && a.splits > 1) {
         const bool live_f = f < a.feats;
 #pragma unroll 1
@@ -1357,6 +1416,56 @@ void make_ext(PArgs& a, const LowParts& lp, int planes) {
             }
 }
 
+// The launch of a plan made as far as split or pairs (run).
+template <class T, bool TR, bool DROP, bool LONG>
+void run_sums(const ProjectTc& p, const Operands& o, PArgs& a, bool split, int sms, cudaStream_t st) {
+    if (!split) {
+        a.n_ft = (int)ceil_div(p.feats, 256);
+        // Columns a tile (steps of 32, an MMA's over a pair): the fewest cycles of a pair's turns,
+        // about 1.1 a step of K for each of the 256 features and np rows that it loads (L2 bounds the
+        // main loop), and for a tile's end 2500, and 30 a row where no second sum hides the epilogue.
+        const int pairs = sms / 2;
+        const int64_t steps = (int64_t)a.kchunks * a.n_terms;
+        int64_t best = -1;
+        for (int np = kMaxColumns<DROP, LONG>; np >= 96; np -= 32) {
+            const int64_t turns = ceil_div(ceil_div(p.rows, np) * a.n_ft, pairs);
+            const int64_t cost = turns * ((np + 256) * steps * 11 / 10 + 2500 + (kSums<DROP, LONG> == 1 ? 30 * np : 0));
+            if (best < 0 || cost < best) {
+                best = cost;
+                a.np = np;
+            }
+        }
+        a.n_mt = (int)ceil_div(p.rows, a.np);
+        a.np = (int)round_up(ceil_div(p.rows, a.n_mt), 32);
+        a.splits = 1;
+    }
+    const int nb = split ? a.np : a.np / 2;   // rows of z a CTA loads
+    const int stage = kTileA + nb * 128;
+    // the join's partial sums, and the CUDA cores' products beside them
+    const int recv = split && a.splits > 1 ? (a.splits + 1) * a.qpo * 2048 : 0;
+    a.stages = std::min(kMaxStages, (kDynMax - 1024 - recv) / stage);
+    const int smem = a.stages * stage + recv + 1024;
+    a.idesc = tc::make_idesc(p.dtype == DT_F16 ? 0u : 1u, TR ? 1u : 0u, 0u, split ? 128 : 256, 0);
+
+    const int wd = p.dtype;
+    CUtensorMap m[4];
+    if (TR) {
+        m[0] = tensor_map(o.W.p, wd, p.feats, p.width, o.W.planes, o.W.ld, o.W.rows * o.W.ld, 64);
+        m[2] = tensor_map(o.Q.p, wd, p.feats, p.rank, o.Q.planes * p.adapters, o.Q.ld, p.rank * o.Q.ld, 64);
+    } else {
+        m[0] = tensor_map(o.W.p, wd, p.width, p.feats, o.W.planes, o.W.ld, o.W.rows * o.W.ld, 128);
+        m[2] = tensor_map(o.Q.p, wd, p.rank, p.feats, o.Q.planes * p.adapters, o.Q.ld, p.feats * o.Q.ld, 128);
+    }
+    m[1] = tensor_map(o.z.p, wd, p.width, p.rows, o.z.planes, o.z.ld, o.z.rows * o.z.ld, nb);
+    const int64_t pc = (int64_t)kPartSlots * a.part_cols;
+    m[3] = tensor_map(p.low.parts, wd, pc, p.rows, 1, pc, p.rows * pc, nb);
+    if (split) {
+        launch(project_split_kernel<T, TR, DROP, LONG>, a.n_ft * a.n_mt * a.splits, kThreads, a.splits, smem, st, m, a);
+    } else {
+        const int pairs = (int)std::min<int64_t>(sms / 2, (int64_t)a.n_ft * a.n_mt);
+        launch(project_pair_kernel<T, TR, DROP, LONG>, 2 * pairs, 64 + 32 * kPairEpi<LONG>, 2, smem, st, m, a);
+    }
+}
 template <class T, bool TR, bool DROP>
 void run(const ProjectTc& p, const Operands& o, cudaStream_t st) {
     PArgs a = {};
@@ -1398,51 +1507,13 @@ void run(const ProjectTc& p, const Operands& o, cudaStream_t st) {
         const int most = a.n_terms > 1 ? a.kchunks : a.kchunks / 2;
         a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({8, sms / tiles_s, most}));
         a.qpo = (int)ceil_div(a.np / 4, a.splits);
-    } else {
-        a.n_ft = (int)ceil_div(p.feats, 256);
-        // Columns a tile (steps of 32, an MMA's over a pair): the fewest cycles of a pair's turns,
-        // about 1.1 a step of K for each of the 256 features and np rows that it loads (L2 bounds the
-        // main loop), and for a tile's end 2500, and 30 a row where no second sum hides the epilogue.
-        const int pairs = sms / 2;
-        const int64_t steps = (int64_t)a.kchunks * a.n_terms;
-        int64_t best = -1;
-        for (int np = kMaxColumns<T, DROP>; np >= 96; np -= 32) {
-            const int64_t turns = ceil_div(ceil_div(p.rows, np) * a.n_ft, pairs);
-            const int64_t cost = turns * ((np + 256) * steps * 11 / 10 + 2500 + (kSums<T, DROP> == 1 ? 30 * np : 0));
-            if (best < 0 || cost < best) {
-                best = cost;
-                a.np = np;
-            }
-        }
-        a.n_mt = (int)ceil_div(p.rows, a.np);
-        a.np = (int)round_up(ceil_div(p.rows, a.n_mt), 32);
-        a.splits = 1;
     }
-    const int nb = split ? a.np : a.np / 2;   // rows of z a CTA loads
-    const int stage = kTileA + nb * 128;
-    // the join's partial sums, and the CUDA cores' products beside them
-    const int recv = split && a.splits > 1 ? (a.splits + 1) * a.qpo * 2048 : 0;
-    a.stages = std::min(kMaxStages, (kDynMax - 1024 - recv) / stage);
-    const int smem = a.stages * stage + recv + 1024;
-    a.idesc = tc::make_idesc(p.dtype == DT_F16 ? 0u : 1u, TR ? 1u : 0u, 0u, split ? 128 : 256, 0);
-
-    const int wd = p.dtype;
-    CUtensorMap m[4];
-    if (TR) {
-        m[0] = tensor_map(o.W.p, wd, p.feats, p.width, o.W.planes, o.W.ld, o.W.rows * o.W.ld, 64);
-        m[2] = tensor_map(o.Q.p, wd, p.feats, p.rank, o.Q.planes * p.adapters, o.Q.ld, p.rank * o.Q.ld, 64);
+    // sums longer than an accumulator's (fp32's are always taken to be)
+    if constexpr (sizeof(T) == 4) {
+        run_sums<T, TR, DROP, true>(p, o, a, split, sms, st);
     } else {
-        m[0] = tensor_map(o.W.p, wd, p.width, p.feats, o.W.planes, o.W.ld, o.W.rows * o.W.ld, 128);
-        m[2] = tensor_map(o.Q.p, wd, p.rank, p.feats, o.Q.planes * p.adapters, o.Q.ld, p.feats * o.Q.ld, 128);
-    }
-    m[1] = tensor_map(o.z.p, wd, p.width, p.rows, o.z.planes, o.z.ld, o.z.rows * o.z.ld, nb);
-    const int64_t pc = (int64_t)kPartSlots * lp.cols;
-    m[3] = tensor_map(p.low.parts, wd, pc, p.rows, 1, pc, p.rows * pc, nb);
-    if (split) {
-        launch(project_split_kernel<T, TR, DROP>, a.n_ft * a.n_mt * a.splits, kThreads, a.splits, smem, st, m, a);
-    } else {
-        const int pairs = (int)std::min<int64_t>(sms / 2, (int64_t)a.n_ft * a.n_mt);
-        launch(project_pair_kernel<T, TR, DROP>, 2 * pairs, 64 + 32 * kPairEpi<T>, 2, smem, st, m, a);
+        if (ceil_div(a.kchunks, split ? a.splits : 1) > kPromote<T>) run_sums<T, TR, DROP, true>(p, o, a, split, sms, st);
+        else run_sums<T, TR, DROP, false>(p, o, a, split, sms, st);
     }
 }
 

@@ -263,3 +263,46 @@ def test_numbers_between_the_products_are_whole(dtype, rank, M, length):
     for k, v in (("y", y), ("dx", dx)):
         worst = float((v.double().abs().amax(1) / bound).max())
         assert worst <= 1.0, f"{k}: {worst:.3g} times its bound"
+
+
+def _ones_like_sums(dtype, M, K, N, R, seed=0):
+    """Positive operands, whose sums a truncation always pulls the same way; adapters of one type and size."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = TYPES[dtype]
+    u = lambda *s, f=1.0: (torch.rand(*s, generator=g, device="cuda") * f).to(t)  # noqa: E731
+    return dict(x=u(M, K), W=u(N, K, f=1 / K), A=u(1, R, K, f=1 / K), B=u(1, N, R, f=1 / R), dy=u(M, N, f=1 / N),
+                ids=torch.zeros(M, dtype=torch.int32, device="cuda"))
+
+
+# How far a sum of positive numbers may be off, whatever its length. Products and additions on the tensor cores are
+# each off by at most 2^-23 of the sum so far (truncated), so a piece of n columns, whose sum grows evenly, by
+# n / 2 * 2^-23 of its value, and the sum of all pieces (rounded to nearest, 2^-24 times the square root of their number)
+# by as much: fp32's pieces are 512 columns, 16-bit types' 4096. (Without pieces 2^20 columns may be off by 2^-4, and
+# were by 2^-10.)
+LONG_FP32 = 512 / 2 * 2.0**-23
+LONG_16 = 4096 / 2 * 2.0**-23
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,K,N", [(8, 1 << 20, 128), (130, 1 << 17, 264), (40, 20000, 2056), (700, 60000, 1700), (2000, 9000, 2056)])
+def test_long_sums_of_the_shared_product(dtype, M, K, N):
+    """Sums over up to 2^20 columns, forward and backward, with no adapter at work: rounded once from a sum
+    that is off by no more than the bounds above."""
+    L = _lora()
+    rows = min(M, 64)
+    eps = torch.finfo(TYPES[dtype]).eps / 2
+    held = LONG_FP32 if dtype == "fp32" else LONG_16
+    for back in (False, True):
+        c = _ones_like_sums(dtype, M, K if not back else N, N if not back else K, 8)
+        c["ids"].fill_(-1)
+        if back:
+            got = L.multi_lora_backward(c["dy"], None, c["W"], c["A"], c["B"], c["ids"], None, want_adapters=False)["dx"]
+            z, W = c["dy"][:rows], c["W"]
+        else:
+            got = L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"])
+            z, W = c["x"][:rows], c["W"].T
+        want = torch.zeros(rows, N, dtype=torch.float64, device="cuda")
+        for k in range(0, K, 16384):
+            want += z[:, k:k + 16384].double() @ W[k:k + 16384].double()
+        off = ((got[:rows].double() - want).abs() - eps * want - (2.0**-25 if dtype == "fp16" else 0)) / want
+        assert float(off.max()) <= held, f"{'dx' if back else 'y'}: off by {float(off.max()):.3g}, bound {held:.3g}"
