@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
         const int ad = sad[pass];
         const float f = a.drop.scale * (a.scale ? a.scale[ad] : 1.f);
         for (int rb = 0; rb < a.rank; rb += NT * 8) {
-            float acc[MT][NT][4] = {};
+            float acc[MT][NT][4] = {}, sum[MT][NT][4] = {};
             // Lane pointers at this warp's first chunk of 64 columns; a turn advances them by 512
             // (a CTA).
             // (Rows of other adapters, or the last row again past the end, are read and their
@@ -492,9 +492,26 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
                             }
                 }
             };
-            int k0 = first * 64;
+            // The sums of kTurns turns, rounded to nearest. (An MMA truncates its sum, always towards zero.)
+            auto gather = [&]() {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            sum[i][n][j] += acc[i][n][j];
+                            acc[i][n][j] = 0.f;
+                        }
+            };
+            constexpr int kTurns = PL == 1 ? 8 : 1;
+            int k0 = first * 64, left = kTurns;
 #pragma unroll 1
             for (; k0 + 64 <= a.width; k0 += turn) {
+                if (left-- == 0) {
+                    gather();
+                    left = kTurns - 1;
+                }
                 step(k0, 0, std::false_type{});
                 step(k0 + 32, 32, std::false_type{});
 #pragma unroll
@@ -508,6 +525,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
                 step(k0, 0, std::true_type{});
                 if (k0 + 32 < a.width) step(k0 + 32, 32, std::true_type{});
             }
+            gather();
             // the warps' sums, in a fixed order: w + (w + 4), then the four; then the CTAs'
             auto at = [&](int i, int n, int j) -> float& {
                 return sums[warp & 3][i * 16 + (j >> 1) * 8 + g][n * 8 + t * 2 + (j & 1)];
@@ -518,7 +536,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) at(i, n, j) = acc[i][n][j];
+                        for (int j = 0; j < 4; ++j) at(i, n, j) = sum[i][n][j];
             __syncthreads();
             if (warp < 4)
 #pragma unroll
@@ -526,7 +544,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) at(i, n, j) += acc[i][n][j];
+                        for (int j = 0; j < 4; ++j) at(i, n, j) += sum[i][n][j];
             __syncthreads();
             auto four = [&](int row, int c) {
                 return (sums[0][row][c] + sums[1][row][c]) + (sums[2][row][c] + sums[3][row][c]);

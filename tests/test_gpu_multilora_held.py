@@ -306,3 +306,36 @@ def test_long_sums_of_the_shared_product(dtype, M, K, N):
             want += z[:, k:k + 16384].double() @ W[k:k + 16384].double()
         off = ((got[:rows].double() - want).abs() - eps * want - (2.0**-25 if dtype == "fp16" else 0)) / want
         assert float(off.max()) <= held, f"{'dx' if back else 'y'}: off by {float(off.max()):.3g}, bound {held:.3g}"
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,K,R", [(8, 1 << 20, 8), (64, 1 << 18, 16), (1100, 20000, 16), (1100, 60000, 40), (2000, 4096, 8)])
+def test_long_sums_of_the_thin_products(dtype, M, K, R):
+    """h over up to 2^20 columns, and g (by dA of one row whose x is one): sums of positive numbers off by no more than
+    2^-23 of themselves for each of a piece's additions, half of that as the piece grows: 512 columns a piece
+    beside 16-bit operands, 64 of six plane products beside fp32 ones, split over eight warps; the pieces, at most
+    2^11, rounded to nearest, 2^-24 each in the root of their number."""
+    L = _lora()
+    pieces = (384 if dtype == "fp32" else 512) / 2 * 2.0**-23 + 2.0**5.5 * 2.0**-24
+    c = _ones_like_sums(dtype, M, K, 64, R)
+    c["W"].zero_()
+    h = torch.empty(M, R, device="cuda")
+    L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"], h=h)
+    rows = min(M, 64)
+    want = torch.zeros(rows, R, dtype=torch.float64, device="cuda")
+    for k in range(0, K, 16384):
+        want += c["x"][:rows, k:k + 16384].double() @ c["A"][0, :, k:k + 16384].double().T
+    off = float(((h[:rows].double() - want) / want).abs().max())
+    assert off <= pieces, f"h: off by {off:.3g}, bound {pieces:.3g}"
+    # g of row 3 alone: x is zero in the others, and each column of dA is then g
+    c = _ones_like_sums(dtype, M, 64, K, R)
+    c["x"].zero_()
+    c["x"][3] = 1
+    dA = L.multi_lora_backward(c["dy"], c["x"], torch.zeros_like(c["W"]), c["A"], c["B"], c["ids"], None, want_dx=False,
+                               want_adapters=False, dA=torch.empty_like(c["A"]))["dA"]
+    want = torch.zeros(R, dtype=torch.float64, device="cuda")
+    for k in range(0, K, 16384):
+        want += c["B"][0, k:k + 16384].double().T @ c["dy"][3, k:k + 16384].double()
+    eps = torch.finfo(TYPES[dtype]).eps / 2
+    off = ((dA[0].double() - want[:, None]).abs() - (2.0**-25 if dtype == "fp16" else 0)) / want[:, None] - eps
+    assert float(off.max()) <= pieces + 2.0**-21, f"g: off by {float(off.max()):.3g}"
