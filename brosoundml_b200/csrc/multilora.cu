@@ -864,11 +864,12 @@ __device__ __forceinline__ uint32_t tf32_hi(float v) {
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
     return r;
 }
-// v = hi + lo in tf32 (22 bits); a number that is not finite has no remainder
+// v = hi + lo in tf32, off by at most 2^-23 (fp32 itself: 2^-24; a third part would be another MMA for every
+// two); a number that is not finite has no remainder, and one that rounds over the range's end is cut
 __device__ __forceinline__ void tf32_split(float v, uint32_t& hi, uint32_t& lo) {
     hi = tf32_hi(v);
-    const float d = v - __uint_as_float(hi);
-    lo = isfinite(v) ? __float_as_uint(d) : 0u;
+    if (isinf(__uint_as_float(hi)) && isfinite(v)) hi = __float_as_uint(v) & 0xFFFFE000u;
+    lo = isfinite(v) ? tf32_hi(v - __uint_as_float(hi)) : 0u;
 }
 __device__ __forceinline__ void mma_1688(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -956,7 +957,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
             if (next >= P.adapters) break;
             ad = next;
         }
+        // An MMA truncates its sum, always towards zero, so those of kPiece steps go to `kept`, rounded to nearest:
+        // fp32's at hand, 16-bit types' (whose long pieces few calls fill) in local memory, having no registers left.
+        constexpr int kPiece = F32 ? 8 : 128;
         float acc[V * NB / 2][2][4] = {};
+        std::conditional_t<F32, float, volatile float> kept[V * NB / 2][2][4];
+        if (F32)
+#pragma unroll
+            for (int i = 0; i < V * NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kept[i >> 1][i & 1][e] = 0.f;
+        int in_piece = 0, pieces = 0;
         int rows_seen = 0;
         for (int base = begin; base < end; base += kList) {
             // the rows of this adapter, in order
@@ -1030,6 +1041,18 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
                 for (int i = 0; i < C::kAhead - 1; ++i) fetch(sg * 8 + i * by, i);
 #pragma unroll 1
             for (int s = sg * 8; s < have; s += by) {
+                if (in_piece++ == kPiece) {
+#pragma unroll
+                    for (int i = 0; i < V * NB; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float& d = acc[i >> 1][i & 1][e];
+                            kept[i >> 1][i & 1][e] = F32 || pieces ? kept[i >> 1][i & 1][e] + d : d;
+                            d = 0.f;
+                        }
+                    in_piece = 1;
+                    pieces = 1;
+                }
                 uint4 q[2][NB];
                 float tv[2][2];
                 if (o.vec) {
@@ -1102,7 +1125,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
                             float(&d)[4] = acc[i * V + j][n];
-                            if constexpr (F32) mma_1688(d, fl, bh[n][0], bh[n][1]);
+                            if constexpr (F32) {
+                                mma_1688(d, fl, bl[n][0], bl[n][1]);
+                                mma_1688(d, fl, bh[n][0], bh[n][1]);
+                            }
                             mma_1688(d, f, bl[n][0], bl[n][1]);
                             mma_1688(d, f, bh[n][0], bh[n][1]);
                         }
@@ -1114,6 +1140,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
             if (tid == 0 && c0 == 0) P.seen[(which * P.adapters + ad) * P.windows + win] = rows_seen;
             if (rows_seen == 0) return;   // (in a window of its own adapter alone)
         }
+        if (F32 || pieces)
+#pragma unroll
+            for (int i = 0; i < V * NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i >> 1][i & 1][e] += kept[i >> 1][i & 1][e];
         // join the step groups; then (column, rank) to the output or the window's partial sums
         __syncthreads();
 #pragma unroll

@@ -339,3 +339,53 @@ def test_long_sums_of_the_thin_products(dtype, M, K, R):
     eps = torch.finfo(TYPES[dtype]).eps / 2
     off = ((dA[0].double() - want[:, None]).abs() - (2.0**-25 if dtype == "fp16" else 0)) / want[:, None] - eps
     assert float(off.max()) <= pieces + 2.0**-21, f"g: off by {float(off.max()):.3g}"
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,R,nA", [(1 << 20, 8, 1), (1 << 20, 8, 100), (200000, 100, 1), (3000, 40, 2)])
+def test_long_sums_of_the_adapters_gradients(dtype, M, R, nA):
+    """dA and dB over up to 2^20 rows of one adapter, positive numbers: off by their output's rounding and 2^-23 of
+    the sum for each of a piece's additions, half of that as the piece grows (64 rows of four products for
+    fp32, 1024 of two for 16-bit types, whose 2^-23 of g and h are within), and 2^-22 for an fp32 product's operands;
+    the pieces, at most 2^11 a warp and 2^8 warps' sums, rounded to nearest. g is a power of two, exactly."""
+    L, t = _lora(), TYPES[dtype]
+    K = N = 64
+    held = (64 * 4 if dtype == "fp32" else 1024 * 2) / 2 * 2.0**-23 + 2.0**-22 + 2.0**-19
+    g = torch.Generator(device="cuda").manual_seed(R)
+    x, dy = torch.rand(M, K, generator=g, device="cuda").to(t), torch.rand(M, N, generator=g, device="cuda").to(t)
+    h = torch.rand(M, R, generator=g, device="cuda") / M
+    ids = torch.full((M,), nA - 1, dtype=torch.int32, device="cuda")
+    W, A = torch.zeros(N, K, dtype=t, device="cuda"), torch.zeros(nA, R, K, dtype=t, device="cuda")
+    B = torch.zeros(nA, N, R, dtype=t, device="cuda")
+    B[:, 0] = 1
+    dy[:, 0] = 0.5
+    scale = torch.full((nA,), 1.0 / M, device="cuda")
+    got = L.multi_lora_backward(dy, x, W, A, B, ids, h, scale=scale, want_dx=False)
+    gr = 0.5 * float(scale[0])
+    want_A = sum(x[i:i + 65536].double().sum(0) for i in range(0, M, 65536)) * gr
+    want_B = sum(dy[i:i + 65536].double().T @ h[i:i + 65536].double() for i in range(0, M, 65536))
+    eps = torch.finfo(t).eps / 2
+    for k, v, w in (("dA", got["dA"][nA - 1], want_A[None].expand(R, -1)), ("dB", got["dB"][nA - 1], want_B)):
+        off = float(((v.double() - w).abs() / w).max()) - eps
+        assert off <= held, f"{k}: off by {off:.3g} more than its rounding, bound {held:.3g}"
+    assert not got["dA"][:nA - 1].any() and not got["dB"][:nA - 1].any()
+
+
+def test_numbers_at_the_end_of_the_range():
+    """fp32's largest numbers times small ones are finite in every output."""
+    L = _lora()
+    M, K, N, R = 40, 640, 264, 8
+    big = torch.finfo(torch.float32).max
+    c = dict(_ones_like_sums("fp32", M, K, N, R), W=torch.full((N, K), 1e-12, device="cuda"))
+    c["A"].fill_(1e-12)
+    c["B"].fill_(1e-12)
+    c["x"].fill_(big)
+    h = torch.empty(M, R, device="cuda")
+    y = L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"], h=h)
+    assert float((y.double() / (big * K * 1e-12) - 1).abs().max()) < 2.0**-18   # (W's and A's own roundings, fp32 sums)
+    dy = torch.full((M, N), 1e-6, device="cuda")
+    dA = L.multi_lora_backward(dy, c["x"], c["W"], c["A"], c["B"], c["ids"], h, want_dx=False)["dA"]
+    assert float((dA.double() / (M * big * N * 1e-18) - 1).abs().max()) < 2.0**-18
+    dy.fill_(big)
+    dB = L.multi_lora_backward(dy, c["x"], c["W"], c["A"], c["B"], c["ids"], torch.full_like(h, 1e-12), want_dx=False)["dB"]
+    assert float((dB.double() / (M * big * 1e-12) - 1).abs().max()) < 2.0**-18
