@@ -19,7 +19,8 @@
 // Every MMA truncates the accumulator's sum, always towards zero: positive fp16 numbers lose 6e-9 of
 // their sum a column (measured: 4e-4 over 65536 columns; fp32's planes 8e-4 over 131072). So long sums leave
 // the accumulator for registers, where fp32 adds round to nearest: fp32's every 512 columns of a pass
-// (9e-7), 16-bit types' every 4096 (2e-5, 1/20 of an fp16 output's rounding).
+// (9e-7), 16-bit types' where an output would feel it, at 1/20 of its rounding: fp16's every 4096 columns
+// (2e-5), bf16's every 16384 (1e-4). (Every 1024 would cost 4 % of 8192 x 4096 x 4096, under dropout 42.)
 #include "multilora_tc.h"
 
 #include <cuda_bf16.h>
@@ -56,7 +57,7 @@ constexpr int kThreads = 320;         // split kernel: TMA warp, MMA warp, 8 epi
 constexpr int kMaxTerms = 6;
 // K steps of 64 in one accumulator, where sums are longer
 template <class T>
-constexpr int kPromote = sizeof(T) == 4 ? 8 : 64;
+constexpr int kPromote = sizeof(T) == 4 ? 8 : std::is_same<T, __half>::value ? 64 : 256;
 constexpr int kMaxExt = 12;
 
 // One TMA stage of the low-rank K steps: 64 ranks of Q plane `plane` from rank `rank0`, 64
@@ -447,13 +448,14 @@ struct Ring {
 };
 
 // Accumulators of a pair, and columns of its tile. TMEM's 512 columns hold two sums, or with dropout
-// (whose low-rank product has an accumulator of its own) one sum and that. Where a tile has many sums (LONG),
-// there are two beside that of the low-rank product. (16-bit with two of 160 columns: 244 us where one of
-// 256, its epilogue not hidden, takes 200: 8192 x 4096 x 4096, 16 ranks. L2 bounds narrow tiles.)
-template <bool DROP, bool LONG>
-constexpr int kSums = DROP && !LONG ? 1 : 2;
-template <bool DROP, bool LONG>
-constexpr int kMaxColumns = DROP && LONG ? 160 : 256;
+// (whose low-rank product has an accumulator of its own) one sum and that. fp32's sums are many a
+// tile, so it has two beside that of the low-rank product. (16-bit with two of 160 columns: 244 us
+// where one of 256, its epilogue not hidden, takes 200: 8192 x 4096 x 4096, 16 ranks. L2 bounds
+// narrow tiles.)
+template <class T, bool DROP>
+constexpr int kSums = DROP && sizeof(T) == 2 ? 1 : 2;
+template <class T, bool DROP>
+constexpr int kMaxColumns = DROP && sizeof(T) == 4 ? 160 : 256;
 // Epilogue warps of a pair's CTA. Many sums run in 16 columns x groups registers a
 // thread: 16 warps of 64 sums (and at most 96 registers) hold 256 columns.
 template <bool LONG>
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
                         const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mT,
                         const __grid_constant__ PArgs a) {
     constexpr bool F16 = std::is_same<T, __half>::value;
-    constexpr int B = kSums<DROP, LONG>;             // sums in TMEM
+    constexpr int B = kSums<T, DROP>;             // sums in TMEM
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accf[2], acce[2], mdone;
@@ -727,7 +729,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
                 u.used(i);
             };
             if constexpr (LONG) {
-                constexpr int NG = (kMaxColumns<DROP, LONG> / 16 + HG - 1) / HG;   // this warp's column groups
+                constexpr int NG = (kMaxColumns<T, DROP> / 16 + HG - 1) / HG;   // this warp's column groups
                 uint32_t powers = 0;
                 if (F16 && (DROP || own)) powers = (uint32_t)load_powers<NG, HG>(a, m0, h, lane);
                 float v[NG][16] = {};
@@ -1427,9 +1429,9 @@ void run_sums(const ProjectTc& p, const Operands& o, PArgs& a, bool split, int s
         const int pairs = sms / 2;
         const int64_t steps = (int64_t)a.kchunks * a.n_terms;
         int64_t best = -1;
-        for (int np = kMaxColumns<DROP, LONG>; np >= 96; np -= 32) {
+        for (int np = kMaxColumns<T, DROP>; np >= 96; np -= 32) {
             const int64_t turns = ceil_div(ceil_div(p.rows, np) * a.n_ft, pairs);
-            const int64_t cost = turns * ((np + 256) * steps * 11 / 10 + 2500 + (kSums<DROP, LONG> == 1 ? 30 * np : 0));
+            const int64_t cost = turns * ((np + 256) * steps * 11 / 10 + 2500 + (kSums<T, DROP> == 1 ? 30 * np : 0));
             if (best < 0 || cost < best) {
                 best = cost;
                 a.np = np;

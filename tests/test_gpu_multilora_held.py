@@ -277,10 +277,9 @@ def _ones_like_sums(dtype, M, K, N, R, seed=0):
 # How far a sum of positive numbers may be off, whatever its length. Products and additions on the tensor cores are
 # each off by at most 2^-23 of the sum so far (truncated), so a piece of n columns, whose sum grows evenly, by
 # n / 2 * 2^-23 of its value, and the sum of all pieces (rounded to nearest, 2^-24 times the square root of their number)
-# by as much: fp32's pieces are 512 columns, 16-bit types' 4096. (Without pieces 2^20 columns may be off by 2^-4, and
+# by as much: fp32's pieces are 512 columns, fp16's 4096, bf16's 16384. (Without pieces 2^20 columns may be off by 2^-4, and
 # were by 2^-10.)
-LONG_FP32 = 512 / 2 * 2.0**-23
-LONG_16 = 4096 / 2 * 2.0**-23
+LONG = {"fp32": 512 / 2 * 2.0**-23, "fp16": 4096 / 2 * 2.0**-23, "bf16": 16384 / 2 * 2.0**-23}
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -291,7 +290,7 @@ def test_long_sums_of_the_shared_product(dtype, M, K, N):
     L = _lora()
     rows = min(M, 64)
     eps = torch.finfo(TYPES[dtype]).eps / 2
-    held = LONG_FP32 if dtype == "fp32" else LONG_16
+    held = LONG[dtype]
     for back in (False, True):
         c = _ones_like_sums(dtype, M, K if not back else N, N if not back else K, 8)
         c["ids"].fill_(-1)
