@@ -49,6 +49,26 @@ __device__ __forceinline__ void report(int gave_up) {
     if (gave_up != tc::TC_OK) atomicCAS(&g_ml_err, tc::TC_OK, gave_up);
 }
 
+// tc::mbar_wait for a role that waits, through others, for one that waits for the kernel before (which may
+// take as long as it likes): the limit counts from that kernel's end.
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, int* err, int code) {
+    const uint64_t t0 = tc::global_timer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        if ((i & 255) == 0) {
+            if (*(volatile int*)err != tc::TC_OK) return false;
+            if (tc::global_timer_ns() - t0 > tc::kWaitLimitNs) break;
+        }
+    }
+    tc::grid_dependency_wait();
+    return tc::mbar_wait(bar, parity, err, code);
+}
+template <bool LONG>
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err, int code) {
+    if (!LONG) return tc::mbar_wait(bar, parity, err, code);   // one sum a tile: no role waits so
+    return tc::mbar_try_wait(bar, parity) || wait_longer(bar, parity, err, code);
+}
+
 constexpr int kSmemMax = 232448;      // opt-in shared memory per block, static and dynamic
 constexpr int kDynMax = kSmemMax - 1024;   // of it dynamic, at most: the kernels' limit, whatever a call takes
 constexpr int kTileA = 16384;         // 128 features x 128 bytes of K
@@ -554,7 +574,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
         bool ok = true, dep = false;
         auto stage = [&](const CUtensorMap* mA, const CUtensorMap* mB, int f0, int ka, int pa, int kb, int row,
                          int pb) {
-            if (!tc::mbar_wait(&empty[r.slot], r.phase ^ 1, err, tc::TC_ERR_WAIT_EMPTY)) return false;
+            if (!wait_for<LONG>(&empty[r.slot], r.phase ^ 1, err, tc::TC_ERR_WAIT_EMPTY)) return false;
             if (rank == 0) tc::mbar_arrive_expect_tx(&full[r.slot], 2 * stage_bytes);
             load_stage<TR, true>(smem + r.slot * stage_bytes, mA, mB, nullptr,
                                  tc::map_shared(tc::smem_u32(&full[r.slot]), 0), f0, ka, pa, kb, row, pb);
@@ -604,7 +624,7 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
             bool ok = true, dep = false;
             Turns u;
             auto vacant = [&](int i) {   // accumulator i is read out
-                return tc::mbar_wait(&acce[i], u.phase(i) ^ 1, err, tc::TC_ERR_WAIT_ACC);   // (at first: at once)
+                return wait_for<LONG>(&acce[i], u.phase(i) ^ 1, err, tc::TC_ERR_WAIT_ACC);   // (at first: at once)
             };
             for (int tile = pair; ok && tile < n_tiles; tile += pairs) {
                 const int m0 = tile_pos(a, tile).m * a.np;
@@ -973,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int issued = head;
         bool ok = true;
         auto stage = [&](const CUtensorMap* mA, const CUtensorMap* mB, int ka, int pa, int kb, int row, int pb) {
-            if (!tc::mbar_wait(&empty[r.slot], r.phase ^ 1, err, tc::TC_ERR_WAIT_EMPTY)) return false;
+            if (!wait_for<LONG>(&empty[r.slot], r.phase ^ 1, err, tc::TC_ERR_WAIT_EMPTY)) return false;
             tc::mbar_arrive_expect_tx(&full[r.slot], stage_bytes);
             load_stage<TR, false>(smem + r.slot * stage_bytes, mA, mB, &full[r.slot], 0, f0, ka, pa, kb, row, pb);
             r.next(a.stages);
@@ -1013,7 +1033,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int s = 0; ok && s < sums; ++s) {
                 const int n = LONG ? min(steps - s * kPromote<T>, kPromote<T>) : steps;
                 const uint32_t d = tbase + (uint32_t)((s & 1) * 128);
-                if (LONG && s >= 2) ok = tc::mbar_wait(&acce[s & 1], (s / 2 - 1) & 1, err, tc::TC_ERR_WAIT_ACC);
+                if (LONG && s >= 2) ok = wait_for<LONG>(&acce[s & 1], (s / 2 - 1) & 1, err, tc::TC_ERR_WAIT_ACC);
                 for (int c = 0; ok && c < n; ++c) {
                     ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
                     if (!ok) break;
