@@ -281,21 +281,21 @@ __global__ void __launch_bounds__(kThreads, 4) shrink_rows_kernel(const __grid_c
     float h = r < r1 ? f * sums[0][r] : 0.f;
     if (r < r1) a.low.t[m * a.rank + r] = h;
     if constexpr (std::is_same<T, __half>::value) {
-        // the row's largest number: over the warps, and the cluster of the row's CTAs
+        // the row's largest number: of the first warp, or over the warps, and the cluster of the row's CTAs
         __shared__ float most[4];
-        if (warp < 4) {
-            const float v = warp_max(finite_size(h));
-            if (lane == 0) most[warp] = v;
-        }
         const int ctas = (int)gridDim.y;
-        if (ctas > 1) tc::cluster_sync();
-        else __syncthreads();
-        float all = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-        if (ctas > 1) {
-            float v = 0.f;   // lane: warp (lane & 3) of CTA lane / 4
-            if (lane < 4 * ctas) v = tc::ld_cluster(tc::map_shared(tc::smem_u32(&most[lane & 3]), lane >> 2));
-            all = warp_max(v);
-            tc::cluster_sync();   // no CTA ends before the others have read it
+        float all = warp < 4 ? warp_max(finite_size(h)) : 0.f;
+        if (a.rank > 32 || ctas > 1) {
+            if (warp < 4 && lane == 0) most[warp] = all;
+            if (ctas > 1) tc::cluster_sync();
+            else __syncthreads();
+            all = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+            if (ctas > 1) {
+                float v = 0.f;   // lane: warp (lane & 3) of CTA lane / 4
+                if (lane < 4 * ctas) v = tc::ld_cluster(tc::map_shared(tc::smem_u32(&most[lane & 3]), lane >> 2));
+                all = warp_max(v);
+                tc::cluster_sync();   // no CTA ends before the others have read it
+            }
         }
         const int power = row_power(all);
         h *= row_factor(power);

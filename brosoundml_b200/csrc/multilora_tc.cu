@@ -328,35 +328,41 @@ __device__ __forceinline__ void add_many(const PArgs& a, int m0, int n, uint32_t
     }
 }
 
+// The products of 4 rows of a group of many adapters, kept ones, for feature f. Whole warp. Not inlined: the
+// registers that it takes would spill around the K loop's end, and the L1 is shared memory.
+template <class T, bool TR, bool DROP>
+__device__ __noinline__ void quad_products(const PArgs& a, int m0, int4 ads, int f, float4* out) {
+    static_assert(kBatch == 4, "a quad of columns");
+    const RngKey key = DROP ? load_rng(a.rng) : RngKey{};
+    if (f >= a.feats) return;
+    const int ad[kBatch] = {ads.x, ads.y, ads.z, ads.w};
+    int m[kBatch];
+    float s[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) m[j] = min(m0 + j, a.rows - 1);
+    low_dots<T, TR>(a, m, ad, f, s);
+    if (DROP)
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (!(keep_bits(f >> 3, (uint32_t)m[j], key, a.drop.thr) >> (f & 7) & 1)) s[j] = 0.f;
+    *out = make_float4(s[0], s[1], s[2], s[3]);
+}
+
 // What the CUDA cores do to 16 rows: the products of a group of many adapters. Not inlined: long, and
 // rarely reached.
 template <class T, bool TR>
 __device__ __noinline__ void many_rows(const PArgs& a, int m0, uint32_t live, uint32_t keep, int f, float* v) {
     add_many<T, TR>(a, m0, 16, live, keep, f, v);
 }
-// Low-rank products of n rows of a mixed group: those not finite, which may be a neighbour's doing,
-// by themselves. (At most the work of a group of many adapters, whatever stands in the operands: the
-// MMAs wait for it, and their waits are bounded.)
+// The low-rank products of 16 rows of a mixed group, each by itself, over those at taddr, some of which are not
+// finite (which may be a neighbour's doing). Whole warp. (The work of a group of many adapters, whatever
+// stands in the operands: others wait for it, and their waits are bounded.)
 template <class T, bool TR>
-__device__ __noinline__ void own_rows(const PArgs& a, int m0, int n, uint32_t live, int f, float* e) {
+__device__ __noinline__ void repair(const PArgs& a, uint32_t live, uint32_t taddr, int m0, int f) {
     float w[16] = {};
-    add_many<T, TR>(a, m0, n, live, 0xFFFFu, f, w);
-    for (int j = 0; j < n; ++j)
-        if (!isfinite(e[j])) e[j] = w[j];
-}
-template <class T, bool TR, int N>
-__device__ __forceinline__ void own_low(const PArgs& a, int gid, int m0, uint32_t live, int f, float (&e)[N]) {
-    if (gid != kMixed) return;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < N; ++j) bad |= !isfinite(e[j]);
-    if (!bad) return;
-    float w[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = e[j];
-    own_rows<T, TR>(a, m0, N, live, f, w);
-#pragma unroll
-    for (int j = 0; j < N; ++j) e[j] = w[j];
+    add_many<T, TR>(a, m0, 16, live, 0xFFFFu, f, w);
+    __syncwarp();
+    tc::tmem_st16(taddr, w);
 }
 
 // Bits j of the result (j = 0..15): column c0 + j of feature f is kept. Lanes 8i..8i+7 of a
@@ -1058,6 +1064,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; ok && i < n_runs; ++i) {
                     const Run u = runs[1][i];
                     const uint32_t idesc = idesc_n(a.idesc, u.cols);
+                    const bool alone = DROP || u.own;   // in an accumulator of its own
+                    const uint32_t d = (alone ? de : tbase + (LONG ? (uint32_t)((sums - 1) & 1) * 128 : 0u)) + (uint32_t)u.c0;
                     for (int e = 0; e < a.n_ext; ++e) {
                         const ExtStage& x = a.ext[e];
                         ok = tc::mbar_wait(&full[r.slot], r.phase, err, tc::TC_ERR_WAIT_FULL);
@@ -1065,9 +1073,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::tc_fence_after();
                         const uint32_t base = tc::smem_u32(smem + r.slot * stage_bytes);
                         for (int k = 0; k < x.n; ++k)
-                            mma<false>(de + (uint32_t)u.c0, desc_a<TR>(base, x.a[k]),
+                            mma<false>(d, desc_a<TR>(base, x.a[k]),
                                        tc::desc_kmajor_sw128(base + kTileA + x.b[k] * 32), idesc,
-                                       !u.first || (e | k) != 0);
+                                       !alone || !u.first || (e | k) != 0);
                         commit<false>(&empty[r.slot]);
                         r.next(a.stages);
                     }
@@ -1153,21 +1161,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = h; i < quads; i += 2) {
                 const int quad = quad0 + i;
                 if (__shfl_sync(0xffffffffu, rows.gid, quad >> 2) != kMany) continue;
-                int m[kBatch], ad[kBatch];
-                float s[kBatch];
-                static_assert(kBatch == 4, "a quad of columns");
+                int ad[4];
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    m[j] = min(m0 + quad * 4 + j, a.rows - 1);
-                    ad[j] = ad_of(i * 4 + j);
-                }
-                if (f >= a.feats) continue;
-                low_dots<T, TR>(a, m, ad, f, s);
-                if (DROP)
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j)
-                        if (!(keep_bits(f >> 3, (uint32_t)m[j], key, a.drop.thr) >> (f & 7) & 1)) s[j] = 0.f;
-                low[i * 128] = make_float4(s[0], s[1], s[2], s[3]);
+                for (int j = 0; j < 4; ++j) ad[j] = ad_of(i * 4 + j);
+                quad_products<T, TR, DROP>(a, m0 + quad * 4, make_int4(ad[0], ad[1], ad[2], ad[3]), f, low + i * 128);
             }
         uint32_t powers = 0;
         if (F16 && split == 0) powers = (uint32_t)load_powers<NG, 2>(a, m0, h, lane);
@@ -1182,9 +1179,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t v[16], y[16];
                 const int gid = __shfl_sync(0xffffffffu, rows.gid, g);
                 const uint32_t live = __shfl_sync(0xffffffffu, rows.rows, g) & 0xFFFFu;
-                const bool ext = split == 0 && by_mma(gid);
+                const bool ext = split == 0 && (DROP ? by_mma(gid) : apart<T>(gid));
+                const uint32_t low_at = trow + (uint32_t)(kLow + g * 16);
                 tc::tmem_ld16_nowait(trow + (uint32_t)(last + g * 16), v);
-                if (ext) tc::tmem_ld16_nowait(trow + (uint32_t)(kLow + g * 16), y);
+                if (ext) tc::tmem_ld16_nowait(low_at, y);
                 tc::tmem_wait_ld();
                 uint32_t keep = 0xFFFFu;
                 if (DROP && (ext || (a.splits == 1 && gid == kMany))) keep = keep_columns(a, m0 + g * 16, f, lane, key);
@@ -1192,13 +1190,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) s[j] = (LONG ? acc[LONG ? i : 0][j] : 0.f) + __uint_as_float(v[j]);
                 if (ext) {
-                    float e[16];
+                    bool b = false;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) e[j] = __uint_as_float(F16 ? times_power(y[j], powers, j) : y[j]);
-                    own_low<T, TR>(a, gid, m0 + g * 16, live, f, e);
+                    for (int j = 0; j < 16; ++j) {
+                        if (F16) y[j] = times_power(y[j], powers, j);
+                        b |= !isfinite(__uint_as_float(y[j]));
+                    }
+                    if (gid == kMixed && __any_sync(0xffffffffu, b)) {
+                        repair<T, TR>(a, live, low_at, m0 + g * 16, f);
+                        tc::tmem_ld16_nowait(low_at, y);
+                        tc::tmem_wait_ld();
+                    }
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        if (keep >> j & 1) s[j] += e[j];
+                        if (keep >> j & 1) s[j] += __uint_as_float(y[j]);
                 }
                 if (F16) powers >>= 8;
                 if (a.splits == 1) {   // nothing to join
@@ -1530,13 +1535,9 @@ void run(const ProjectTc& p, const Operands& o, cudaStream_t st) {
         a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({8, sms / tiles_s, most}));
         a.qpo = (int)ceil_div(a.np / 4, a.splits);
     }
-    // sums longer than an accumulator's (fp32's are always taken to be)
-    if constexpr (sizeof(T) == 4) {
-        run_sums<T, TR, DROP, true>(p, o, a, split, sms, st);
-    } else {
-        if (ceil_div(a.kchunks, split ? a.splits : 1) > kPromote<T>) run_sums<T, TR, DROP, true>(p, o, a, split, sms, st);
-        else run_sums<T, TR, DROP, false>(p, o, a, split, sms, st);
-    }
+    // Sums longer than an accumulator's? (Of fp32's passes only the last adds numbers of the sum's own size.)
+    if (ceil_div(a.kchunks, split ? a.splits : 1) > kPromote<T>) run_sums<T, TR, DROP, true>(p, o, a, split, sms, st);
+    else run_sums<T, TR, DROP, false>(p, o, a, split, sms, st);
 }
 
 template <class T>
