@@ -608,8 +608,9 @@ __global__ void __launch_bounds__(kThreads) shrink_tile_kernel(const __grid_cons
 // 128 features x 32 rows a CTA on the CUDA cores (true fp32 products), with the rows' h made by
 // every CTA that needs them: at these sizes a launch costs more than the few products. Not
 // worth it beyond: the thin product is repeated for every 128 features, and the wide one runs
-// at the CUDA cores' rate. Bound by latency: one clip's 128 x 2048 fp32 projection 9.8 us, 256 clips'
-// (4.7 MB, 0.15 GFLOP) 14.4.
+// at the CUDA cores' rate. Bound by latency: one clip's 128 x 2048 fp32 projection (rank 8) 9.8 us, 256 clips'
+// (4.7 MB, 0.15 GFLOP) 14.4. (Its rule does not look at the rank: at 128 ranks the thin product is as large as a CTA's
+// wide one. Not measured there.)
 constexpr int kSmallF = 128, kSmallR = 32, kSmallK = 128, kSmallPitch = kSmallK + 4;
 
 struct SmallArgs {
@@ -898,7 +899,7 @@ struct OuterCfg {
 // divide the ranks (16 a warp) and the steps; their sums join in shared memory in warp order.
 // Bound by instructions (operands unpacked, and with dropout the generator's, a third of the time) and
 // the start and join of a CTA's adapters, not by z: 8192 rows, bf16, 16 ranks, dA and dB of 4096
-// columns each (134 MB) 91 us with dropout, about 65 without.
+// columns each (134 MB) 91 us with dropout, 71 without.
 template <class T>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
     outer_kernel(const __grid_constant__ OuterPair P) {

@@ -520,8 +520,9 @@ __device__ __forceinline__ TilePos tile_pos(const PArgs& a, int tile) {
 // Without, groups where adapters meet inside an MMA's columns have it in the accumulator of the next tile's
 // shared sum, and the epilogue adds it to the tile's own, in TMEM, before anything else (Turns).
 // Bound by the tensor pipe at 256 columns (about 560 cycles for 64 columns of K, of which 512 are
-// MMAs), by L2's operand rate below: 8192 x 4096 x 4096 bf16 187 us alone (1.47 PFLOP/s; the low-rank
-// steps of 16 ranks and 8 prompts add 3), 203 with dropout; 2048 x 2048 x 2048 fp32 106 us.
+// MMAs), by L2's operand rate below. A call of 8192 x 4096 x 4096 bf16 with 16 ranks, its thin product (26 us)
+// and all, on the GPU: one adapter 208 us, prompts of 1000 rows 214, of 40 (every group apart) 270, fp16 (always
+// apart) 229, the backward's dx 208, under dropout 231; fp32 2048 x 2048 x 2048 118.
 template <class T, bool TR, bool DROP, bool LONG>
 __global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
     project_pair_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
@@ -923,8 +924,8 @@ __global__ void __launch_bounds__(64 + 32 * kPairEpi<LONG>, 1)
 // cluster's CTAs. Each CTA sends its fp32 partial columns to the CTA that finishes them (qpo
 // quads of columns each) through distributed shared memory; they are summed in CTA order. Bound by
 // reading W once: every SM has a TMA ring of its own share of K in flight. One token of 4096 x 4096
-// bf16 (34 MB) 13 us after a thin product of 5.7 that it overlaps; 64 tokens of 32 requests x 4096 x 8192
-// (81 MB) 25.
+// bf16 (34 MB) 14 us beside a thin product of 5.6 that it overlaps (15.2 in all); 64 tokens of 32 requests x
+// 4096 x 8192 (81 MB) 24 (28.4).
 template <class T, bool TR, bool DROP, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
     project_split_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,

@@ -262,7 +262,9 @@ def multi_lora_forward(x, W, A, B, row_ids, bias=None, scale=None, dropout: floa
     (adapters,) float32, 1 by default. x and y may be rows of a wider tensor. ``y``: given, its padding
     rows are left as they were; else a new tensor, in which they are zero. ``dropout`` > 0 drops the
     adapters' input, with ``rng`` = int64 {seed, offset} on the device. ``h`` (rows, rank) float32, when
-    given, receives what :func:`multi_lora_backward` needs. Works on ``x``'s device and its current stream."""
+    given, receives what :func:`multi_lora_backward` needs. Works on ``x``'s device and its current stream,
+    with scratch of its own that later calls use again (:func:`release_scratch`). A kernel whose bounded wait runs
+    out leaves its outputs incomplete and a code that ``bsml_device_error`` reads."""
     (rows, _), dtype, device = _matrix("x", x)
     shape, cin, cout, rank, W, A, B, ids, scale, rng = _adapter_args(W, A, B, row_ids, scale, dropout, rng, y is None,
                                                                      rows, dtype, device)

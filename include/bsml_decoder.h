@@ -408,7 +408,8 @@ int bsml_convlora_load(bsml_convlora* l, const char* path);
  * cout) with row stride ldy, all of one dtype; scale (adapters, float) or NULL for 1;
  * h (rows, rank, float). Rows do not mix: a NaN or infinity in one row or one
  * adapter stays in the rows of its own. Sums are kept in fp32 and rounded once to
- * the dtype; the tensor cores take h (and the backward's g) as three bf16 numbers, which
+ * the dtype (the tensor cores truncate theirs, in pieces: within 1e-6 of positive
+ * numbers' sum in fp32, 1/20 of a 16-bit output's rounding); the tensor cores take h (and the backward's g) as three bf16 numbers, which
  * hold an fp32 number whole, and beside fp16 operands as two fp16 ones (off by 2^-22, or
  * 2^-39 of the row's largest number). rank is 1..BSML_MULTILORA_MAX_RANK, cin and cout at most 2^20.
  * Dropout of the adapters' input (not of the shared projection's) has probability
