@@ -143,13 +143,14 @@ def test_a_wait_that_ran_out_is_told_and_spoils_no_later_call():
     assert C.bsml_device_error() == 0
 
 
-@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("p", [0.0, 0.1])
 @pytest.mark.parametrize("where", ["W", "x", "A", "B"])
-def test_no_numbers_hold_a_call_up(dtype, where):
+def test_no_numbers_hold_a_call_up(dtype, p, where):
     """A weight, rows or an adapter of NaN among short prompts: the call takes what it takes with ordinary
     numbers, up to the products of the rows beside that adapter on the CUDA cores (a few times as long; the
     shared product again for every element would be hundreds). Rows of the others keep their results."""
-    M, W = (2500, 2048) if dtype == "fp32" else (5000, 4096)
+    M, W = {"fp32": (2500, 2048), "bf16": (5000, 4096), "fp16": (2500, 4500)}[dtype]   # fp16: a tile of several sums
     c = _make(dtype, M, W, W, 8, 5, "short", seed=2)
     bad = {k: v.clone() for k, v in c.items()}
     if where in "AB":
@@ -163,8 +164,11 @@ def test_no_numbers_hold_a_call_up(dtype, where):
     h = torch.empty(M, 8, device="cuda")
 
     def run(c):
-        y = L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"], h=h)
-        return y, L.multi_lora_backward(c["dy"], None, c["W"], c["A"], c["B"], c["ids"], None, want_adapters=False)["dx"]
+        y = L.multi_lora_forward(c["x"], c["W"], c["A"], c["B"], c["ids"], h=h, **kw)
+        return y, L.multi_lora_backward(c["dy"], None, c["W"], c["A"], c["B"], c["ids"], None, want_adapters=False,
+                                        **kw)["dx"]
+
+    kw = dict(dropout=p, rng=_rng() if p else None)
 
     def time(c):
         run(c)

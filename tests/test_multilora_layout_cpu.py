@@ -19,7 +19,7 @@ using namespace bsml;
 int main() {
     int checked = 0, bad = 0;
     for (int at : {4096, 4098, 4104})
-        for (long long rows : {1ll, 2ll, 7ll, 64ll})
+        for (long long rows : {1ll, 2ll, 3ll, 7ll, 64ll})
             for (int rank = 1; rank <= 128; ++rank)
                 for (bool f32 : {false, true}) {
                     const Operand o = operand((const void*)(size_t)at, rank, rows, rank, f32, true);
@@ -48,4 +48,4 @@ def test_no_piece_reaches_past_an_operand(tmp_path):
     subprocess.run([cxx, "-std=c++17", "-Wall", "-Wextra", "-I", os.path.join(ROOT, "brosoundml_b200", "csrc"),
                     str(src), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True)
-    assert out.returncode == 0 and out.stdout == "3072 checked, 0 bad\n", out.stdout
+    assert out.returncode == 0 and out.stdout.endswith(" checked, 0 bad\n"), out.stdout
